@@ -343,6 +343,145 @@ int tl_kv_append_rope_q8(const tl_kv_layer_q8 *L, const float *k, const float *v
                          uint32_t kv_stride, const uint32_t *slots, uint32_t pos,
                          uint32_t n, const tl_rope_params *rope, void *stream);
 
+/* ---- batches of chunks over a paged cache ---------------------------------
+ * One call for the new rows of several sessions: some bring one token, some a
+ * chunk of a prompt.  The sessions' rows lie in one pool (a tl_kv_layer or
+ * tl_kv_layer_q8), in pages of page_size rows (a power of two; 1: the slot
+ * tables of the entry points above), and one batch buffer holds all new rows.
+ * Position p of a session is row
+ *     pages[p / page_size] * page_size + p % page_size
+ * of the pool, or row p when the session has no table.  A table covers the
+ * positions [0, pos + n).  Pages outside the pool: the rows of an append are
+ * skipped, the keys of an attention are not seen.
+ * Sessions may share pages that they only read; a page that receives new rows
+ * belongs to one chunk of the call.  Ring layers have no pages and are refused.
+ * At most 4096 chunks, positions below 2^31.
+ *
+ * Batch rows that belong to no chunk, and the columns past a row's heads, are
+ * neither read nor written.  Pointers are of the current device; the calls
+ * work in order on `stream`, keep no reference to their host arguments and
+ * hold no state between them.  q, k and v rows are f32 and 16-byte aligned.
+ * (No counterpart in the reference, which runs one session per call,
+ * src/backend/cpu/cpu_op.c:964-1064; its head norm and its rotation are ops of
+ * their own, cpu_op.c:632-700.)
+ */
+#define TL_MAX_PAGE 4096
+typedef struct tl_chunk {
+    const uint32_t *pages;    /* device: the session's page table; NULL = identity (one chunk
+                                 per call only) */
+    uint32_t  pos;            /* position of its first new row */
+    uint32_t  n;              /* its new rows (0: the chunk is skipped) */
+    uint32_t  row;            /* batch row of the first one; chunks share no rows */
+    uint32_t  prefix;         /* attention: keys at positions [0, prefix) are seen by every row,
+                                 also by earlier ones and past the window (0: none) */
+    uint32_t  rope_skip;      /* append: rotations are of position + rope_skip (positions that
+                                 the session has evicted so far) */
+    uint32_t  pad_;
+    float    *weight;         /* tl_attn_weight: device [pos + n], added to */
+} tl_chunk;
+
+/* Norm of queries and keys for each head, rotation and append in one pass:
+ *     y = x / sqrt(mean(x^2) + eps) * weight      over each head's head_dim
+ * for every head of q and k, then the rotation `rope` (as tl_rope_params, the
+ * angle reduced in 64 bits), q to q_out, and the new K and V rows into the
+ * cache (V as it is).  q_out may be q. */
+typedef struct tl_qk_norm_args {
+    const float *q;           /* device [rows][q_stride] */
+    const float *k;           /* device [rows][kv_stride] */
+    const float *v;           /* device [rows][kv_stride] */
+    float       *q_out;       /* device [rows][q_out_stride] */
+    const float *q_weight;    /* device [head_dim]; NULL = ones */
+    const float *k_weight;    /* device [head_dim]; NULL = ones */
+    float        eps;         /* >= 0 */
+    uint32_t     rows;        /* rows of the batch buffers */
+    uint32_t     n_head;      /* a multiple of n_kv_head */
+    uint32_t     q_stride;    /* floats between rows, multiples of 4 */
+    uint32_t     kv_stride;
+    uint32_t     q_out_stride;
+    uint32_t     page_size;
+    tl_rope_params rope;      /* rope_dim 0: no rotation */
+} tl_qk_norm_args;
+int tl_qk_norm_append(const tl_kv_layer *L, const tl_qk_norm_args *a, const tl_chunk *chunks,
+                      uint32_t n_chunk, void *stream);
+int tl_qk_norm_append_q8(const tl_kv_layer_q8 *L, const tl_qk_norm_args *a,
+                         const tl_chunk *chunks, uint32_t n_chunk, void *stream);
+
+/* Attention of the chunks' rows over the cache (which holds the new rows
+ * already), in f32 accuracy: q and the probabilities are taken as pairs of
+ * f16, so their rounding is that of 22 bits.  A row at position p sees key j
+ *     (j <= p and (window == 0 or p - j < window)) or j < prefix
+ *     and j >= first[row] and j < pos + n
+ * and its score is
+ *     s = scale * q.k;  softcap > 0: s = softcap * tanh(s / softcap)
+ *     slopes: s -= slopes[head] * |p - j|
+ * A row that sees nothing gives zeros, and a log sum of -infinity.  Keys that
+ * a row does not see have no part in it, whatever their K and V hold; a key
+ * that it does see should be finite. */
+typedef struct tl_chunk_attn_args {
+    const float    *q;        /* device [rows][q_stride], rotated */
+    float          *dst;      /* device [rows][q_stride] */
+    float          *lse;      /* device [rows][n_head]: log(sum(exp(s))) of each row and head;
+                                 NULL: not wanted */
+    const uint32_t *first;    /* device [rows]: first position that a row sees (the start of its
+                                 document); NULL = 0 */
+    const float    *slopes;   /* device [n_head]; NULL = no distance bias */
+    uint32_t        rows;     /* rows of the batch buffers */
+    uint32_t        n_head;   /* a multiple of n_kv_head */
+    uint32_t        q_stride; /* floats between q / dst rows, a multiple of 4 */
+    uint32_t        page_size;
+    uint32_t        window;   /* 0 = all */
+    float           scale;    /* > 0 */
+    float           softcap;  /* 0 = none */
+    void           *ws;       /* device workspace of this call, 16-byte aligned, zeroed before its
+                                 first use and used by one call at a time; NULL = the stream's
+                                 own (not under HIP graph capture) */
+    uint64_t        ws_bytes; /* at least tl_attn_chunks_ws() */
+} tl_chunk_attn_args;
+int tl_attn_chunks(const tl_kv_layer *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                   uint32_t n_chunk, void *stream);
+int tl_attn_chunks_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a,
+                      const tl_chunk *chunks, uint32_t n_chunk, void *stream);
+/* Bytes of workspace that tl_attn_chunks / tl_attn_weight (either cache) need
+ * for these chunks. */
+int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl_chunk_attn_args *a,
+                      const tl_chunk *chunks, uint32_t n_chunk, uint64_t *bytes);
+
+/* The attention weight that the chunks' rows gave to every position of their
+ * sessions: for each chunk and each position j < pos + n
+ *     weight[j] += sum over its rows and all heads of exp(s - lse)
+ * with the scores and masks of tl_attn_chunks, whose lse these are (dst is not
+ * used).  The order of the sums is fixed: equal calls give equal bits. */
+int tl_attn_weight(const tl_kv_layer *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                   uint32_t n_chunk, void *stream);
+int tl_attn_weight_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a,
+                      const tl_chunk *chunks, uint32_t n_chunk, void *stream);
+
+/* Eviction by accumulated attention weight: of a session's `len` positions the
+ * first `sink`, the last `recent` and those of largest weight stay, `keep` in
+ * all (equal weights: the lower position stays; NaN counts as less than any
+ * number, -0 as 0).  Writes the kept positions in rising order, the pool rows
+ * that hold them (in a cache of single-row pages the session's new table; in
+ * one of larger pages the source rows of a tl_kv_copy into new pages), the
+ * rows of the evicted positions in the order of their positions, and the kept
+ * weights.  The pool's rows themselves are not touched.  After it the session
+ * has `keep` positions, and rope_skip grows by len - keep. */
+typedef struct tl_evict_seq {
+    const float    *weight;   /* device [len] */
+    const uint32_t *pages;    /* device: the session's page table; NULL = identity */
+    uint32_t        len;
+    uint32_t        keep;     /* 1 .. len */
+    uint32_t        sink;     /* sink + recent <= keep */
+    uint32_t        recent;
+    uint32_t        page_size;
+    uint32_t        pad_;
+    uint32_t       *kept;     /* device [keep]; NULL: not wanted */
+    uint32_t       *rows;     /* device [keep]; NULL: not wanted */
+    uint32_t       *freed;    /* device [len - keep]; NULL: not wanted */
+    float          *weight_out; /* device [keep]; NULL: not wanted.  No output may overlap an
+                                   input or another output */
+} tl_evict_seq;
+int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *stream);
+
 /* Measurement aid (no reference counterpart): stream `bytes` of device
  * memory with 16-byte loads, `depth` (1/4/8/16) in flight per lane, over
  * `blocks` workgroups of 256; sink receives blocks*256 words.  Gives the

@@ -1,0 +1,384 @@
+/* tl_chunk.h — launch blocks and device helpers of the calls on batches of
+ * chunks over a paged cache (include/tlkv.h, tl_chunk). */
+#pragma once
+#include "tl_common.h"
+#include "tl_internal.h"
+
+#define CK_MAX_SEQ 32          /* chunks of one launch; longer batches take several */
+#define CK_MAX_CHUNKS 4096     /* chunks of one call */
+#define CK_KEYS 32             /* keys of one tile */
+#define CK_COLS 16             /* (row, head) columns of one narrow tile */
+
+/* Split merge: one arrival counter per group, zero between launches, at the
+ * start of the workspace; (max, sum) pairs and partial rows follow. */
+#define CK_MAX_GROUPS 4096
+#define CK_CNT_PAD 4
+#define CK_CNT_WORDS (CK_MAX_GROUPS * CK_CNT_PAD)
+static_assert(CK_CNT_WORDS <= TL_MERGE_CNT_WORDS, "counters of a stream's workspace");
+
+/* One chunk of a launch: its workgroups are [wg0, next wg0), ncb column blocks
+ * x n_kv heads x ns key splits of them; part0 / grp0: its first partial row
+ * set and merge counter (ns > 1). */
+struct CkSeq {
+    const u32 *pages;
+    float *weight;
+    u32 pos, n, row, prefix, rope_skip;
+    u32 wg0, ncb, ns, part0, grp0;
+};
+
+struct CkCache {
+    const u16 *k, *v;          /* f16 rows, or int8 rows of a Q8_0 cache */
+    const u16 *ks, *vs;        /* Q8_0 scales */
+    u32 cap, n_kv, shift;      /* page_size = 1 << shift */
+};
+
+struct CkAttnParams {
+    CkSeq seq[CK_MAX_SEQ];
+    CkCache c;
+    const float *q;
+    float *dst, *lse;
+    const u32 *first;
+    const float *slopes;
+    u32 n_seq, n_head, gqa, q_stride, window;
+    float scale, softcap;
+    float *ws_acc;
+    float2 *ws_ml;
+    u32 *cnt;
+};
+
+/* host side (tl_chunk.hip) */
+int tl_chunk_check(const LayerView &L, const tl_chunk *chunks, u32 n_chunk, u32 rows,
+                   u32 page_size, u32 *shift);
+int tl_check_layer(const tl_kv_layer *L);
+int tl_check_layer_q8(const tl_kv_layer_q8 *L);
+LayerView tl_view_q8(const tl_kv_layer_q8 *L);
+bool tl_ranges_overlap(const void *a, u64 a_bytes, const void *b, u64 b_bytes);
+
+/* ---- device ---------------------------------------------------------------- */
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef u32 u4_t __attribute__((ext_vector_type(4)));
+
+#define CK_LOG2E 1.4426950408889634f
+#define CK_LN2 0.6931471805599453f
+
+/* pool row of a session's position; ~0 where its page lies outside the pool */
+TL_DEV u32 ck_row(const CkCache &c, const u32 *pages, u32 p) {
+    if (!pages) return p;
+    const u32 pg = pages[p >> c.shift];
+    return pg <= c.cap >> c.shift ? (pg << c.shift) + (p & ((1u << c.shift) - 1)) : ~0u;
+}
+
+/* index of the launch's chunk that workgroup b belongs to (wg0 rises) */
+TL_DEV u32 ck_find(const CkSeq *seq, u32 n_seq, u32 b) {
+    const u32 lane = threadIdx.x & 63;
+    const bool le = lane < n_seq && seq[lane].wg0 <= b;
+    return (u32)__builtin_amdgcn_readfirstlane((int)__popcll(__ballot(le)) - 1);
+}
+
+/* exp(2|x|) based above 1/4 ((e - 1) / (e + 1): the subtraction is exact to
+ * the rounding of e), the odd series below, so the result is good to a few
+ * units of its last place over the whole range */
+TL_DEV float ck_tanh(float x) {
+    const float ax = fabsf(x), x2 = x * x;
+    const float e = __builtin_amdgcn_exp2f(fminf(ax, 10.f) * (2.f * CK_LOG2E));
+    const float big = copysignf((e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f), x);
+    float s = fmaf(x2, 62.f / 2835.f, -17.f / 315.f);
+    s = fmaf(x2, s, 2.f / 15.f);
+    s = fmaf(x2, s, -1.f / 3.f);
+    const float small = fmaf(x * x2, s, x);
+    return ax < 0.25f ? small : big;
+}
+
+/* f32 as a pair of f16 whose sum has 22 bits of it */
+TL_DEV void ck_split(float x, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16)x;
+    lo = (_Float16)(x - (float)hi);
+}
+
+/* power of two that brings a row's largest |x| to [2^14, 2^15), so that both
+ * halves of every element that matters are normal f16 numbers: exponent of it
+ * (rows of zeros, infinities or NaN: any) */
+TL_DEV int ck_row_exp(float amax) {
+    const int e = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127;
+    return 14 - (e < -100 ? -100 : e > 126 ? 126 : e);
+}
+
+/* Which keys a (row, head) column sees: [lo, lo + w) and [f, f + pw). */
+struct CkSees {
+    u32 lo, w, f, pw, hi, pre;
+    TL_DEV void set(u32 p, u32 end, u32 window, u32 prefix, u32 first) {
+        f = first;
+        pre = prefix < end ? prefix : end;
+        hi = p + 1;
+        lo = window && hi > window ? hi - window : 0;
+        lo = lo > f ? lo : f;
+        w = hi > lo ? hi - lo : 0;
+        pw = pre > f ? pre - f : 0;
+    }
+    TL_DEV bool sees(u32 key) const { return key - lo < w || key - f < pw; }
+};
+
+template <int N>
+TL_DEV u32 group_umin(u32 x) {
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) {
+        const u32 y = __shfl_xor(x, o);
+        x = y < x ? y : x;
+    }
+    return x;
+}
+template <int N>
+TL_DEV u32 group_umax(u32 x) {
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) {
+        const u32 y = __shfl_xor(x, o);
+        x = y > x ? y : x;
+    }
+    return x;
+}
+TL_DEV u32 ck_uniform(u32 x) { return (u32)__builtin_amdgcn_readfirstlane((int)x); }
+
+/* The key tiles that a block of columns needs: [a0, a0 + na) of the prefix,
+ * then nb from b0 on.  full(): every column sees every key of a tile. */
+struct CkTiles {
+    u32 a0, na, b0, nb;
+    u32 max_lo, min_hi, max_f, pre;
+    /* N: lanes over which the columns lie (the other lanes repeat them) */
+    template <int N>
+    TL_DEV void set(const CkSees &s) {
+        const u32 none = 0xffffffffu;
+        const u32 fmin = ck_uniform(group_umin<N>(s.pw ? s.f : none));
+        const u32 lo = ck_uniform(group_umin<N>(s.w ? s.lo : none));
+        const u32 hi = ck_uniform(group_umax<N>(s.w ? s.hi : 0));
+        max_lo = ck_uniform(group_umax<N>(s.lo));
+        min_hi = ck_uniform(group_umin<N>(s.hi));
+        max_f = ck_uniform(group_umax<N>(s.f));
+        pre = ck_uniform(s.pre);
+        a0 = na = b0 = nb = 0;
+        if (fmin != none) {
+            a0 = fmin / CK_KEYS;
+            na = (pre + CK_KEYS - 1) / CK_KEYS - a0;
+        }
+        if (lo != none) {
+            b0 = lo / CK_KEYS;
+            u32 b1 = (hi + CK_KEYS - 1) / CK_KEYS;
+            if (na && b0 < a0 + na) b0 = a0 + na;
+            nb = b1 > b0 ? b1 - b0 : 0;
+        }
+    }
+    TL_DEV u32 count() const { return na + nb; }
+    TL_DEV u32 key(u32 t) const { return (t < na ? a0 + t : b0 + (t - na)) * CK_KEYS; }
+    TL_DEV bool full(u32 kb) const {
+        return (kb >= max_lo && kb + CK_KEYS <= min_hi) || (kb >= max_f && kb + CK_KEYS <= pre);
+    }
+};
+
+/* ---- one wave's tile of 32 keys x 16 columns, operands straight from memory --
+ *
+ * S^T[key][col] = K . Q^T and O^T[dim][col] += V^T . P^T run on
+ * v_mfma_f32_16x16x32_f16.  Lane (i = lane & 15, g = lane >> 4):
+ *   K  two sub-tiles a: row i of the matrix is key 8 * (i >> 2) + 4 * a + (i & 3),
+ *      k-step s the dims 32 s + 8 g ..: one 16-byte load each;
+ *   S  so the accumulators of sub-tile a hold keys 8 g + 4 a + r of column i:
+ *      a lane's eight scores are keys 8 g .. 8 g + 7, which is the order in
+ *      which the second product takes them (k index 8 g + e);
+ *   V  the lane loads dims (D / 16) i .. of those eight keys, whole rows per 16
+ *      lanes; matrix m takes the m-th of its dims: eight halves picked from
+ *      eight registers, one v_perm per pair.  No transposing pass over LDS.
+ * A Q8_0 element is int8 x f16, 18 bits: taken as a pair hi + lo of f16 (the
+ * product's rounding and its exact remainder). */
+template <int D>
+struct CkTileF16 {
+    static constexpr int KS = D / 32, DW = D / 32;   /* k-steps; V dwords per key and lane */
+    u4_t kr[2][KS];
+    u32 vr[8][DW];
+    TL_DEV void load_k(const CkCache &c, u32 kvh, const u32 (&rk)[2], u32 g) {
+        const char *base = (const char *)(c.k + (u64)kvh * c.cap * D);
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                kr[a][s] = *(const u4_t *)(base + (u64)(rk[a] * (u32)(D * 2) + s * 64 + g * 16));
+    }
+    TL_DEV void load_v(const CkCache &c, u32 kvh, const u32 (&rv)[8], u32 i) {
+        const char *base = (const char *)(c.v + (u64)kvh * c.cap * D);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const char *r = base + (u64)(rv[e] * (u32)(D * 2) + i * (D / 8));
+            if constexpr (DW == 2) {
+                const uint2 x = *(const uint2 *)r;
+                vr[e][0] = x.x;
+                vr[e][1] = x.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < DW / 4; j++) {
+                    const u4_t x = *(const u4_t *)(r + 16 * j);
+                    vr[e][4 * j] = x[0];
+                    vr[e][4 * j + 1] = x[1];
+                    vr[e][4 * j + 2] = x[2];
+                    vr[e][4 * j + 3] = x[3];
+                }
+            }
+        }
+    }
+    static constexpr bool LO = false;
+    TL_DEV void get_k(int a, int s, h8_t &hi, h8_t &) const { hi = __builtin_bit_cast(h8_t, kr[a][s]); }
+    TL_DEV void get_v(int m, h8_t &hi, h8_t &) const {
+        u4_t x;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            x[j] = __builtin_amdgcn_perm(vr[2 * j + 1][m >> 1], vr[2 * j][m >> 1],
+                                         m & 1 ? 0x07060302u : 0x05040100u);
+        hi = __builtin_bit_cast(h8_t, x);
+    }
+    TL_DEV void clear_v(int e) {
+#pragma unroll
+        for (int d = 0; d < DW; d++) vr[e][d] = 0;
+    }
+    TL_DEV bool odd_v(int e) const {      /* key e holds infinities or NaN */
+        bool b = false;
+#pragma unroll
+        for (int d = 0; d < DW; d++)
+            b |= (vr[e][d] & 0x7c00u) == 0x7c00u || (vr[e][d] & 0x7c000000u) == 0x7c000000u;
+        return b;
+    }
+};
+
+/* int8 pairs x scale as f16 pairs hi + lo */
+TL_DEV void ck_q8_pair(tl_half2 v, tl_half2 d, u32 &hi, u32 &lo) {
+    const tl_half2 h = v * d;
+    const tl_half2 l = __builtin_elementwise_fma(v, d, -h);
+    hi = __builtin_bit_cast(u32, h);
+    lo = __builtin_bit_cast(u32, l);
+}
+
+template <int D>
+struct CkTileQ8 {
+    static constexpr int KS = D / 32, NB = D / 16;   /* k-steps; V bytes per key and lane */
+    uint2 kr[2][KS];
+    u32 sk[2][KS / 2];
+    u32 vr[8][NB / 4];
+    u16 sv[8];
+    TL_DEV void load_k(const CkCache &c, u32 kvh, const u32 (&rk)[2], u32 g) {
+        const char *base = (const char *)c.k + (u64)kvh * c.cap * D;
+        const char *sb = (const char *)(c.ks + (u64)kvh * c.cap * KS);
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                kr[a][s] = *(const uint2 *)(base + (u64)(rk[a] * (u32)D + s * 32 + g * 8));
+#pragma unroll
+            for (int s = 0; s < KS / 2; s++)
+                sk[a][s] = *(const u32 *)(sb + (u64)(rk[a] * (u32)(KS * 2) + s * 4));
+        }
+    }
+    TL_DEV void load_v(const CkCache &c, u32 kvh, const u32 (&rv)[8], u32 i) {
+        const char *base = (const char *)c.v + (u64)kvh * c.cap * D;
+        const char *sb = (const char *)(c.vs + (u64)kvh * c.cap * KS);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const char *r = base + (u64)(rv[e] * (u32)D + i * NB);
+            if constexpr (NB == 4) {
+                vr[e][0] = *(const u32 *)r;
+            } else if constexpr (NB == 8) {
+                const uint2 x = *(const uint2 *)r;
+                vr[e][0] = x.x;
+                vr[e][1] = x.y;
+            } else {
+                const u4_t x = *(const u4_t *)r;
+#pragma unroll
+                for (int j = 0; j < 4; j++) vr[e][j] = x[j];
+            }
+            sv[e] = *(const u16 *)(sb + (u64)(rv[e] * (u32)(KS * 2) + i * NB / 32 * 2));
+        }
+    }
+    static constexpr bool LO = true;
+    TL_DEV void get_k(int a, int s, h8_t &hi, h8_t &lo) const {
+        const u32 d = (sk[a][s >> 1] >> (16 * (s & 1))) & 0xffffu;
+        const tl_half2 d2 = __builtin_bit_cast(tl_half2, d * 0x10001u);
+        tl_half2 v[4];
+        i8x4_to_f16(kr[a][s].x, v[0], v[1]);
+        i8x4_to_f16(kr[a][s].y, v[2], v[3]);
+        u4_t h, l;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            u32 x, y;
+            ck_q8_pair(v[j], d2, x, y);
+            h[j] = x;
+            l[j] = y;
+        }
+        hi = __builtin_bit_cast(h8_t, h);
+        lo = __builtin_bit_cast(h8_t, l);
+    }
+    TL_DEV void get_v(int m, h8_t &hi, h8_t &lo) const {
+        u4_t h, l;
+        const u32 sel = 0x0c000c00u | (u32)(m & 3) | ((u32)(4 + (m & 3)) << 16);
+        const tl_half2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            /* byte m of keys 2j and 2j + 1: q + 128 under the exponent of 1024 */
+            const u32 b = __builtin_amdgcn_perm(vr[2 * j + 1][m >> 2], vr[2 * j][m >> 2], sel);
+            const tl_half2 v = __builtin_bit_cast(tl_half2, (b ^ 0x00800080u) | 0x64006400u) - bias;
+            u32 x, y;
+            ck_q8_pair(v, __builtin_bit_cast(tl_half2, (u32)sv[2 * j] | ((u32)sv[2 * j + 1] << 16)), x, y);
+            h[j] = x;
+            l[j] = y;
+        }
+        hi = __builtin_bit_cast(h8_t, h);
+        lo = __builtin_bit_cast(h8_t, l);
+    }
+    TL_DEV void clear_v(int e) { sv[e] = 0; }
+    TL_DEV bool odd_v(int e) const { return (sv[e] & 0x7fffu) > 0x6006u; }   /* 127 d past f16 */
+};
+
+template <int D, bool Q8>
+struct CkTile;
+template <int D>
+struct CkTile<D, false> : CkTileF16<D> {};
+template <int D>
+struct CkTile<D, true> : CkTileQ8<D> {};
+
+/* q of a column as f16 pairs, scaled by its row's power of two; returns the
+ * factor that takes the products back to scale * q.k */
+template <int D>
+TL_DEV float ck_load_q(const float *qrow, u32 g, float scale, h8_t (&hi)[D / 32], h8_t (&lo)[D / 32]) {
+    float x[D / 32][8];
+    float m = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 32; s++) {
+        const float4 a = *(const float4 *)(qrow + 32 * s + 8 * g);
+        const float4 b = *(const float4 *)(qrow + 32 * s + 8 * g + 4);
+        x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
+        x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+        m = fmaxf(m, amax8(x[s]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const int e = ck_row_exp(m);
+    const float up = __uint_as_float((u32)(e + 127) << 23);
+    const float down = __uint_as_float((u32)(127 - e) << 23);
+#pragma unroll
+    for (int s = 0; s < D / 32; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            _Float16 h, l;
+            ck_split(x[s][j] * up, h, l);
+            hi[s][j] = h;
+            lo[s][j] = l;
+        }
+    return down * scale;
+}
+
+/* the eight scores of a lane from its products, in units of log2 */
+template <bool BIAS>
+TL_DEV float ck_score(float s, float cs, float softcap, float icap, float slope, u32 p, u32 key) {
+    float x = s * cs;
+    if constexpr (BIAS) {
+        if (softcap > 0.f) x = softcap * ck_tanh(x * icap);
+        x = fmaf(-slope, (float)(p > key ? p - key : key - p), x);
+        x *= CK_LOG2E;
+    }
+    return x;
+}

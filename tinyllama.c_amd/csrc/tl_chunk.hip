@@ -1,0 +1,566 @@
+/*
+ * tl_chunk.hip — batches of chunks over a paged cache: checks of arguments,
+ * the norm + rotation + append of new rows, and the entry points and plans of
+ * the attention (tl_chunk_attn_kernels.h) and of the attention weight
+ * (tl_chunk_weight_kernels.h).
+ */
+#include "tl_chunk.h"
+#include "tl_chunk_launch.h"
+
+#include <math.h>
+#include <string.h>
+
+/* ------------------------------------------------------------------------ */
+/* checks                                                                    */
+/* ------------------------------------------------------------------------ */
+
+bool tl_ranges_overlap(const void *a, u64 a_bytes, const void *b, u64 b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
+/* do the intervals [at(i), at(i) + len(i)) of items with len > 0 overlap?
+ * Rising ones (the usual order) are seen in one pass. */
+template <class At, class Len>
+static bool any_overlap(u32 n, At at, Len len) {
+    u64 end = 0;
+    bool rising = true;
+    for (u32 i = 0; i < n && rising; i++) {
+        if (!len(i)) continue;
+        rising = at(i) >= end;
+        end = at(i) + len(i);
+    }
+    if (rising) return false;
+    for (u32 i = 0; i < n; i++)
+        for (u32 j = 0; j < i; j++)
+            if (len(i) && len(j) && at(i) < at(j) + len(j) && at(j) < at(i) + len(i)) return true;
+    return false;
+}
+
+int tl_chunk_check(const LayerView &L, const tl_chunk *ch, u32 n_chunk, u32 rows, u32 page_size,
+                   u32 *shift) {
+    if (n_chunk > CK_MAX_CHUNKS || (n_chunk && !ch))
+        return tl_fail(TL_EINVAL, "chunks: 0..%d chunks", CK_MAX_CHUNKS);
+    if (!page_size || (page_size & (page_size - 1)) || page_size > TL_MAX_PAGE)
+        return tl_fail(TL_EINVAL, "chunks: page size %u is no power of two up to %d", page_size, TL_MAX_PAGE);
+    *shift = (u32)__builtin_ctz(page_size);
+    if (L.ring) return tl_fail(TL_EINVAL, "chunks: ring layers have no pages");
+    u32 live = 0, bare = 0;
+    for (u32 i = 0; i < n_chunk; i++) {
+        if (!ch[i].n) continue;
+        live++;
+        if ((u64)ch[i].row + ch[i].n > rows)
+            return tl_fail(TL_ERANGE, "chunks: rows %u + %u of chunk %u exceed %u", ch[i].row, ch[i].n, i, rows);
+        if ((u64)ch[i].pos + ch[i].n > 0x7fffffffull ||
+            (u64)ch[i].pos + ch[i].n + ch[i].rope_skip > 0xffffffffull)
+            return tl_fail(TL_ERANGE, "chunks: positions of chunk %u", i);
+        if ((uintptr_t)ch[i].pages & 3) return tl_fail(TL_EINVAL, "chunks: page table of chunk %u not aligned", i);
+        if (!ch[i].pages) {
+            bare++;
+            if ((u64)ch[i].pos + ch[i].n > L.cap)
+                return tl_fail(TL_ERANGE, "chunks: pos %u + n %u exceeds cap %u", ch[i].pos, ch[i].n, L.cap);
+        }
+    }
+    if (bare && live > 1) return tl_fail(TL_EINVAL, "chunks: more than one chunk needs page tables");
+    if (any_overlap(n_chunk, [&](u32 i) { return (u64)ch[i].row; }, [&](u32 i) { return (u64)ch[i].n; }))
+        return tl_fail(TL_EINVAL, "chunks: two chunks share batch rows");
+    return TL_OK;
+}
+
+static CkCache cache_of(const LayerView &L, u32 shift) {
+    CkCache c;
+    c.k = (const u16 *)L.k;
+    c.v = (const u16 *)L.v;
+    c.ks = L.ks;
+    c.vs = L.vs;
+    c.cap = L.cap;
+    c.n_kv = L.n_kv_head;
+    c.shift = shift;
+    return c;
+}
+
+static void seq_of(CkSeq &s, const tl_chunk &c) {
+    memset(&s, 0, sizeof(s));
+    s.pages = c.pages;
+    s.weight = c.weight;
+    s.pos = c.pos;
+    s.n = c.n;
+    s.row = c.row;
+    s.prefix = c.prefix;
+    s.rope_skip = c.rope_skip;
+}
+
+/* rows x stride floats starting at p, of which each row holds `width` */
+static u64 span(u32 rows, u32 stride, u32 width) {
+    return rows ? ((u64)(rows - 1) * stride + width) * sizeof(float) : 0;
+}
+
+static int check_rows(const char *what, const void *p, u32 stride, u64 width) {
+    if (!p) return tl_fail(TL_EINVAL, "chunks: null %s", what);
+    if (stride < width || (stride & 3) || ((uintptr_t)p & 15))
+        return tl_fail(TL_EINVAL, "chunks: %s rows must be 16-byte aligned, of at least %llu floats", what,
+                       (unsigned long long)width);
+    return TL_OK;
+}
+
+/* ------------------------------------------------------------------------ */
+/* norm + rotation + append                                                  */
+/* ------------------------------------------------------------------------ */
+
+struct CkAppendParams {
+    CkSeq seq[CK_MAX_SEQ];
+    CkCache c;
+    const float *q, *k, *v, *qw, *kw;
+    float *q_out;
+    float eps;
+    u32 n_seq, n_head, q_stride, kv_stride, q_out_stride;
+    u32 rdim;
+    int neox;
+    double step;             /* log2(theta) * 2 / rdim */
+};
+
+/* One workgroup per batch row and share of its heads (grid.y): the row's
+ * rotation table goes to LDS once, then every group of D / 8 lanes takes head
+ * rows of q, k and v in turn, eight elements to a lane: sum of squares over
+ * the group by DPP, norm, rotation with the partner's elements (in the lane
+ * for adjacent pairs, from lane +- rdim / 16 for half pairs), store. */
+template <int D, bool Q8>
+__global__ __launch_bounds__(256) void chunk_append_kernel(const CkAppendParams p) {
+    constexpr u32 LPR = D / 8, GRP = 256 / LPR;
+    __shared__ float2 s_cs[D / 2];
+    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const u32 r = blockIdx.x - sq.wg0;
+    const u32 key = sq.pos + r;
+    const u64 brow = (u64)sq.row + r;
+    if (threadIdx.x < p.rdim / 2) {
+        /* turns in 64 bits: the fraction is good at any position */
+        const double turns = (double)(key + sq.rope_skip) * (exp2(-p.step * (double)threadIdx.x) * 0.15915494309189535);
+        float s, c;
+        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+        s_cs[threadIdx.x] = make_float2(c, s);
+    }
+    const u32 prow = ck_row(p.c, sq.pages, key);
+    __syncthreads();
+    const u32 e0 = (threadIdx.x % LPR) * 8;
+    const u32 units = p.n_head + 2 * p.c.n_kv;
+    const u32 half = p.rdim >> 1;
+    for (u32 u = blockIdx.y * GRP + threadIdx.x / LPR; u < units; u += gridDim.y * GRP) {
+        const bool is_q = u < p.n_head, is_v = u >= p.n_head + p.c.n_kv;
+        const u32 h = is_q ? u : is_v ? u - p.n_head - p.c.n_kv : u - p.n_head;
+        const float *src = is_q ? p.q + brow * p.q_stride : is_v ? p.v + brow * p.kv_stride : p.k + brow * p.kv_stride;
+        src += (u64)h * D;
+        const float4 a = *(const float4 *)(src + e0), b = *(const float4 *)(src + e0 + 4);
+        float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
+        ss = group_sum<LPR>(ss);
+        if (!is_v) {
+            const float inv = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+            const float *w = is_q ? p.qw : p.kw;
+            float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+            if (w) {
+                const float4 c = *(const float4 *)(w + e0), d = *(const float4 *)(w + e0 + 4);
+                g[0] = c.x; g[1] = c.y; g[2] = c.z; g[3] = c.w;
+                g[4] = d.x; g[5] = d.y; g[6] = d.z; g[7] = d.w;
+            }
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = x[j] * inv * g[j];
+            if (p.rdim && !p.neox) {
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    if (e0 + j < p.rdim) {
+                        const float2 cs = s_cs[(e0 + j) >> 1];
+                        rope_rot(y[j], y[j + 1], cs.x, cs.y, x[j], x[j + 1]);
+                    } else {
+                        x[j] = y[j];
+                        x[j + 1] = y[j + 1];
+                    }
+            } else if (p.rdim) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const u32 e = e0 + j;
+                    if (e >= p.rdim) {
+                        x[j] = y[j];
+                        continue;
+                    }
+                    const bool low = e < half;
+                    const u32 pe = low ? e + half : e - half;
+                    const float o = src[pe] * inv * (w ? w[pe] : 1.f);
+                    const float2 cs = s_cs[low ? e : pe];
+                    float nx, ny;
+                    rope_rot(low ? y[j] : o, low ? o : y[j], cs.x, cs.y, nx, ny);
+                    x[j] = low ? nx : ny;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = y[j];
+            }
+        }
+        if (is_q) {
+            float *d = p.q_out + brow * p.q_out_stride + (u64)h * D + e0;
+            *(float4 *)d = make_float4(x[0], x[1], x[2], x[3]);
+            *(float4 *)(d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else if constexpr (Q8) {
+            const float m = group_max<4>(amax8(x));
+            const float d = m / 127.f, id = d > 0.f ? 1.f / d : 0.f;
+            if (prow < p.c.cap) {
+                const u64 at = (u64)h * p.c.cap + prow;
+                char *dst = (char *)(is_v ? p.c.v : p.c.k) + at * D + e0;
+                *(uint2 *)dst = q8_pack8(x, id);
+                if ((e0 & 31) == 0)
+                    ((u16 *)(is_v ? p.c.vs : p.c.ks))[at * (D / 32) + (e0 >> 5)] = (u16)f32_to_f16_bits(d);
+            }
+        } else if (prow < p.c.cap) {
+            u16 *dst = (u16 *)(is_v ? p.c.v : p.c.k) + ((u64)h * p.c.cap + prow) * D + e0;
+            *(uint4 *)dst = cvt8_f16_regs(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]));
+        }
+    }
+}
+
+template <bool Q8>
+static void launch_append(u32 head_dim, dim3 grid, hipStream_t st, const CkAppendParams &p) {
+    if (head_dim == 64) hipLaunchKernelGGL((chunk_append_kernel<64, Q8>), grid, dim3(256), 0, st, p);
+    else if (head_dim == 128) hipLaunchKernelGGL((chunk_append_kernel<128, Q8>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((chunk_append_kernel<256, Q8>), grid, dim3(256), 0, st, p);
+}
+
+static int norm_append(const LayerView &L, const tl_qk_norm_args *a, const tl_chunk *ch, u32 n_chunk,
+                       hipStream_t st) {
+    if (!a) return tl_fail(TL_EINVAL, "qk_norm: null arguments");
+    if (!a->n_head || a->n_head % L.n_kv_head)
+        return tl_fail(TL_EINVAL, "qk_norm: n_head %u not a multiple of n_kv %u", a->n_head, L.n_kv_head);
+    const u64 qw = (u64)a->n_head * L.head_dim, kw = (u64)L.n_kv_head * L.head_dim;
+    u32 shift;
+    int rc = tl_chunk_check(L, ch, n_chunk, a->rows, a->page_size, &shift);
+    if (!rc) rc = check_rows("q", a->q, a->q_stride, qw);
+    if (!rc) rc = check_rows("q_out", a->q_out, a->q_out_stride, qw);
+    if (!rc) rc = check_rows("k", a->k, a->kv_stride, kw);
+    if (!rc) rc = check_rows("v", a->v, a->kv_stride, kw);
+    if (rc) return rc;
+    if (((uintptr_t)a->q_weight | (uintptr_t)a->k_weight) & 15)
+        return tl_fail(TL_EINVAL, "qk_norm: weights not 16-byte aligned");
+    if (!(a->eps >= 0.f) || !isfinite(a->eps)) return tl_fail(TL_EINVAL, "qk_norm: eps %g", (double)a->eps);
+    if (a->q_out == a->q ? a->q_out_stride != a->q_stride
+                         : tl_ranges_overlap(a->q, span(a->rows, a->q_stride, (u32)qw), a->q_out,
+                                             span(a->rows, a->q_out_stride, (u32)qw)) &&
+                               /* column blocks of one buffer lie apart in each row */
+                               !(a->q_stride == a->q_out_stride &&
+                                 (u64)((a->q > a->q_out ? a->q - a->q_out : a->q_out - a->q)) >= qw &&
+                                 (u64)((a->q > a->q_out ? a->q - a->q_out : a->q_out - a->q)) + qw <= a->q_stride))
+        return tl_fail(TL_EINVAL, "qk_norm: q_out overlaps q");
+    RopeCfg rope;
+    rope.rdim = 0;
+    if (a->rope.rope_dim) {
+        rc = tl_rope_cfg(L.head_dim, &a->rope, rope);
+        if (rc) return rc;
+        if (!isfinite(a->rope.theta)) return tl_fail(TL_EINVAL, "rope: theta");
+    }
+    CkAppendParams p;
+    memset(&p, 0, sizeof(p));
+    p.c = cache_of(L, shift);
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.qw = a->q_weight;
+    p.kw = a->k_weight;
+    p.q_out = a->q_out;
+    p.eps = a->eps;
+    p.n_head = a->n_head;
+    p.q_stride = a->q_stride;
+    p.kv_stride = a->kv_stride;
+    p.q_out_stride = a->q_out_stride;
+    p.rdim = rope.rdim;
+    p.neox = rope.rdim ? rope.neox : 0;
+    p.step = rope.rdim ? log2((double)rope.theta) * 2.0 / rope.rdim : 0.0;
+    for (u32 i = 0; i < n_chunk;) {
+        u32 m = 0;
+        u64 wgs = 0;
+        for (; i < n_chunk && m < CK_MAX_SEQ; i++) {
+            if (!ch[i].n) continue;
+            if (wgs + ch[i].n > 0x7fffffffull) break;
+            seq_of(p.seq[m], ch[i]);
+            p.seq[m++].wg0 = (u32)wgs;
+            wgs += ch[i].n;
+        }
+        if (!m) break;
+        p.n_seq = m;
+        /* few rows: their heads over several workgroups */
+        const u32 units = a->n_head + 2 * L.n_kv_head, per = 256 / (L.head_dim / 8);
+        u32 split = (units + per - 1) / per;
+        while (split > 1 && wgs * split > 1024) split--;
+        if (L.q8) launch_append<true>(L.head_dim, dim3((u32)wgs, split), st, p);
+        else launch_append<false>(L.head_dim, dim3((u32)wgs, split), st, p);
+        HIP_TRY(hipGetLastError());
+    }
+    return TL_OK;
+}
+
+extern "C" int tl_qk_norm_append(const tl_kv_layer *L, const tl_qk_norm_args *a, const tl_chunk *chunks,
+                                 uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer(L);
+    return rc ? rc : norm_append(tl_view(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+extern "C" int tl_qk_norm_append_q8(const tl_kv_layer_q8 *L, const tl_qk_norm_args *a,
+                                    const tl_chunk *chunks, uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer_q8(L);
+    return rc ? rc : norm_append(tl_view_q8(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+/* ------------------------------------------------------------------------ */
+/* attention                                                                 */
+/* ------------------------------------------------------------------------ */
+
+/* keys that a launch may have to go through for rows [r0, r1) of a chunk (the
+ * documents' starts are known on the device only) */
+static u64 span_tiles(const tl_chunk &c, u32 window, u32 r0, u32 r1) {
+    const u64 end = (u64)c.pos + c.n;
+    const u64 pre = c.prefix < end ? c.prefix : end;
+    const u64 hi = (u64)c.pos + r1;
+    u64 lo = window && (u64)c.pos + r0 + 1 > window ? (u64)c.pos + r0 + 1 - window : 0;
+    if (lo < pre) lo = pre;
+    return (pre + CK_KEYS - 1) / CK_KEYS + (hi > lo ? (hi + CK_KEYS - 1) / CK_KEYS - lo / CK_KEYS : 0);
+}
+
+struct AttnPlan {
+    u32 wgs;           /* workgroups of the launch */
+    u64 sets;          /* partial sets of 16 rows */
+    u32 groups;        /* merge counters */
+};
+
+/* Workgroups of ck_wave tiles: as many splits as fill the chip twice over (two
+ * workgroups to a CU), none of fewer than one tile for each wave. */
+static AttnPlan plan_attn(CkSeq *seq, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 window) {
+    u64 total = 0;
+    u64 tiles[CK_MAX_SEQ];
+    for (u32 i = 0; i < n; i++) {
+        seq[i].ncb = (u32)(((u64)seq[i].n * gqa + CK_COLS - 1) / CK_COLS);
+        tiles[i] = span_tiles(*ch[i], window, 0, ch[i]->n);
+        total += tiles[i] * seq[i].ncb * n_kv;
+    }
+    u64 per = (total + 511) / 512;
+    if (per < 4) per = 4;
+    AttnPlan pl = {0, 0, 0};
+    u64 wgs = 0;
+    for (u32 i = 0; i < n; i++) {
+        u64 ns = (tiles[i] + per - 1) / per;
+        const u64 groups = (u64)seq[i].ncb * n_kv;
+        if (ns < 1 || pl.groups + groups > CK_MAX_GROUPS) ns = 1;
+        seq[i].ns = (u32)ns;
+        seq[i].wg0 = (u32)wgs;
+        seq[i].part0 = (u32)pl.sets;
+        seq[i].grp0 = pl.groups;
+        wgs += groups * ns;
+        if (ns > 1) {
+            pl.sets += groups * ns;
+            pl.groups += (u32)groups;
+        }
+    }
+    pl.wgs = wgs > 0x7fffffffull ? 0 : (u32)wgs;
+    return pl;
+}
+
+#define CK_WS_HEAD ((u64)CK_CNT_WORDS * sizeof(u32))
+static u64 ws_need(u64 sets, u32 head_dim) {
+    return CK_WS_HEAD + sets * CK_COLS * (sizeof(float2) + (u64)head_dim * sizeof(float));
+}
+
+static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
+                      bool weight, u32 *shift) {
+    if (!a) return tl_fail(TL_EINVAL, "attn_chunks: null arguments");
+    if (!a->n_head || a->n_head % L.n_kv_head)
+        return tl_fail(TL_EINVAL, "attn_chunks: n_head %u not a multiple of n_kv %u", a->n_head, L.n_kv_head);
+    const u64 width = (u64)a->n_head * L.head_dim;
+    int rc = tl_chunk_check(L, ch, n_chunk, a->rows, a->page_size, shift);
+    if (!rc) rc = check_rows("q", a->q, a->q_stride, width);
+    if (!rc && !weight) rc = check_rows("dst", a->dst, a->q_stride, width);
+    if (rc) return rc;
+    if (((uintptr_t)a->lse | (uintptr_t)a->first | (uintptr_t)a->slopes) & 3)
+        return tl_fail(TL_EINVAL, "attn_chunks: lse, first or slopes not aligned");
+    if (!(a->scale > 0.f) || !isfinite(a->scale) || !(a->softcap >= 0.f) || !isfinite(a->softcap))
+        return tl_fail(TL_EINVAL, "attn_chunks: scale %g softcap %g", (double)a->scale, (double)a->softcap);
+    if ((uintptr_t)a->ws & 15) return tl_fail(TL_EINVAL, "attn_chunks: workspace not 16-byte aligned");
+    return TL_OK;
+}
+
+/* the call's chunks with rows, at most CK_MAX_SEQ of them from *at on */
+static u32 next_chunks(const tl_chunk *ch, u32 n_chunk, u32 *at, CkSeq *seq, const tl_chunk **of) {
+    u32 m = 0;
+    for (; *at < n_chunk && m < CK_MAX_SEQ; (*at)++)
+        if (ch[*at].n) {
+            seq_of(seq[m], ch[*at]);
+            of[m++] = &ch[*at];
+        }
+    return m;
+}
+
+/* most partial sets that a launch of the call takes */
+static u64 most_sets(u32 n_kv, u32 gqa, u32 window, const tl_chunk *ch, u32 n_chunk) {
+    CkSeq seq[CK_MAX_SEQ];
+    const tl_chunk *of[CK_MAX_SEQ];
+    u64 most = 0;
+    for (u32 i = 0; i < n_chunk;) {
+        const u32 m = next_chunks(ch, n_chunk, &i, seq, of);
+        if (!m) break;
+        const AttnPlan pl = plan_attn(seq, of, m, n_kv, gqa, window);
+        most = pl.sets > most ? pl.sets : most;
+    }
+    return most;
+}
+
+extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl_chunk_attn_args *a,
+                                 const tl_chunk *chunks, uint32_t n_chunk, uint64_t *bytes) {
+    if (!a || !bytes || (n_chunk && !chunks) || n_chunk > CK_MAX_CHUNKS || !n_kv_head || !a->n_head ||
+        a->n_head % n_kv_head || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return tl_fail(TL_EINVAL, "attn_chunks_ws: arguments");
+    *bytes = ws_need(most_sets(n_kv_head, a->n_head / n_kv_head, a->window, chunks, n_chunk), head_dim);
+    return TL_OK;
+}
+
+/* where the call's counters, pairs and partial rows lie (its launches take
+ * them one after another) */
+static int take_ws(const tl_chunk_attn_args *a, u64 sets, u32 head_dim, hipStream_t st, CkAttnParams &p) {
+    if (!sets) return TL_OK;
+    if (sets * CK_COLS * head_dim * sizeof(float) > 0x7ffffff0ull)
+        return tl_fail(TL_ERANGE, "attn_chunks: %llu partial sets", (unsigned long long)sets);
+    if (a->ws) {
+        const u64 need = ws_need(sets, head_dim);
+        if (a->ws_bytes < need)
+            return tl_fail(TL_ERANGE, "attn_chunks: workspace of %llu bytes, %llu needed",
+                           (unsigned long long)a->ws_bytes, (unsigned long long)need);
+        p.cnt = (u32 *)a->ws;
+        p.ws_ml = (float2 *)((char *)a->ws + CK_WS_HEAD);
+        p.ws_acc = (float *)(p.ws_ml + sets * CK_COLS);
+        return TL_OK;
+    }
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(st, &cs));
+    if (cs != hipStreamCaptureStatusNone)
+        return tl_fail(TL_EINVAL, "attn_chunks: a captured call takes its own workspace (ws)");
+    TlWorkspace *w;
+    const int rc = tl_workspace_get(st, sets * CK_COLS * head_dim, sets * CK_COLS, TL_MERGE_CNT_WORDS, &w);
+    if (rc) return rc;
+    p.cnt = w->cnt;
+    p.ws_ml = (float2 *)w->ml;
+    p.ws_acc = w->acc;
+    return TL_OK;
+}
+
+static void fill_attn(CkAttnParams &p, const LayerView &L, const tl_chunk_attn_args *a, u32 shift) {
+    memset(&p, 0, sizeof(p));
+    p.c = cache_of(L, shift);
+    p.q = a->q;
+    p.dst = a->dst;
+    p.lse = a->lse;
+    p.first = a->first;
+    p.slopes = a->slopes;
+    p.n_head = a->n_head;
+    p.gqa = a->n_head / L.n_kv_head;
+    p.q_stride = a->q_stride;
+    p.window = a->window;
+    p.scale = a->scale;
+    p.softcap = a->softcap;
+}
+
+static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
+                       hipStream_t st) {
+    u32 shift;
+    int rc = check_attn(L, a, ch, n_chunk, false, &shift);
+    if (rc) return rc;
+    if (tl_ranges_overlap(a->q, span(a->rows, a->q_stride, a->n_head * L.head_dim), a->dst,
+                          span(a->rows, a->q_stride, a->n_head * L.head_dim)))
+        return tl_fail(TL_EINVAL, "attn_chunks: dst overlaps q");
+    CkAttnParams p;
+    fill_attn(p, L, a, shift);
+    rc = take_ws(a, most_sets(L.n_kv_head, p.gqa, a->window, ch, n_chunk), L.head_dim, st, p);
+    if (rc) return rc;
+    const tl_chunk *of[CK_MAX_SEQ];
+    for (u32 i = 0; i < n_chunk;) {
+        const u32 m = next_chunks(ch, n_chunk, &i, p.seq, of);
+        if (!m) break;
+        p.n_seq = m;
+        const AttnPlan pl = plan_attn(p.seq, of, m, L.n_kv_head, p.gqa, a->window);
+        if (!pl.wgs) return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
+        ck_launch_attn(p, L.head_dim, L.q8, pl.wgs, st);
+        HIP_TRY(hipGetLastError());
+    }
+    return TL_OK;
+}
+
+extern "C" int tl_attn_chunks(const tl_kv_layer *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                              uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer(L);
+    return rc ? rc : attn_chunks(tl_view(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+extern "C" int tl_attn_chunks_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                                 uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer_q8(L);
+    return rc ? rc : attn_chunks(tl_view_q8(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+/* ------------------------------------------------------------------------ */
+/* attention weight                                                          */
+/* ------------------------------------------------------------------------ */
+
+static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
+                       hipStream_t st) {
+    u32 shift;
+    int rc = check_attn(L, a, ch, n_chunk, true, &shift);
+    if (rc) return rc;
+    if (!a->lse) return tl_fail(TL_EINVAL, "attn_weight: null lse");
+    for (u32 i = 0; i < n_chunk; i++)
+        if (ch[i].n && (!ch[i].weight || ((uintptr_t)ch[i].weight & 3)))
+            return tl_fail(TL_EINVAL, "attn_weight: weight of chunk %u", i);
+    if (any_overlap(n_chunk, [&](u32 i) { return (u64)(uintptr_t)ch[i].weight; },
+                    [&](u32 i) { return ch[i].n ? ((u64)ch[i].pos + ch[i].n) * 4 : 0; }))
+        return tl_fail(TL_EINVAL, "attn_weight: two chunks share weights");
+    CkAttnParams p;
+    fill_attn(p, L, a, shift);
+    const tl_chunk *of[CK_MAX_SEQ];
+    for (u32 i = 0; i < n_chunk;) {
+        const u32 m = next_chunks(ch, n_chunk, &i, p.seq, of);
+        if (!m) break;
+        p.n_seq = m;
+        u64 wgs = 0;
+        for (u32 j = 0; j < m; j++) {
+            p.seq[j].wg0 = (u32)wgs;
+            p.seq[j].ncb = (u32)(((u64)p.seq[j].n * p.gqa + CK_COLS - 1) / CK_COLS);
+            wgs += ((u64)p.seq[j].pos + p.seq[j].n + CK_KEYS - 1) / CK_KEYS;
+        }
+        if (wgs > 0x7fffffffull) return tl_fail(TL_ERANGE, "attn_weight: too many keys");
+        ck_launch_weight(p, L.head_dim, L.q8, (u32)wgs, st);
+        HIP_TRY(hipGetLastError());
+    }
+    return TL_OK;
+}
+
+extern "C" int tl_attn_weight(const tl_kv_layer *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                              uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer(L);
+    return rc ? rc : attn_weight(tl_view(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+extern "C" int tl_attn_weight_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
+                                 uint32_t n_chunk, void *stream) {
+    const int rc = tl_check_layer_q8(L);
+    return rc ? rc : attn_weight(tl_view_q8(L), a, chunks, n_chunk, (hipStream_t)stream);
+}
+
+/* ------------------------------------------------------------------------ */
+/* instances                                                                 */
+/* ------------------------------------------------------------------------ */
+
+void ck_launch_attn(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) q8 ? ck_launch_attn_t<64, true>(p, wgs, st) : ck_launch_attn_t<64, false>(p, wgs, st);
+    else if (head_dim == 128) q8 ? ck_launch_attn_t<128, true>(p, wgs, st) : ck_launch_attn_t<128, false>(p, wgs, st);
+    else q8 ? ck_launch_attn_t<256, true>(p, wgs, st) : ck_launch_attn_t<256, false>(p, wgs, st);
+}
+
+void ck_launch_weight(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) q8 ? ck_launch_weight_t<64, true>(p, wgs, st) : ck_launch_weight_t<64, false>(p, wgs, st);
+    else if (head_dim == 128) q8 ? ck_launch_weight_t<128, true>(p, wgs, st) : ck_launch_weight_t<128, false>(p, wgs, st);
+    else q8 ? ck_launch_weight_t<256, true>(p, wgs, st) : ck_launch_weight_t<256, false>(p, wgs, st);
+}

@@ -17,6 +17,7 @@
  */
 #include "tl_common.h"
 #include "tl_internal.h"
+#include "tl_chunk.h"
 #include "../../include/tlkv.h"
 
 #include <atomic>
@@ -939,3 +940,5 @@ extern "C" int tl_probe_read(const void *src, uint64_t bytes, uint32_t *sink,
 
 /* Error reporting for the C translation units of the library. */
 extern "C" int tl_set_error(int code, const char *msg) { return tl_fail(code, "%s", msg); }
+
+int tl_check_layer(const tl_kv_layer *L) { return check_layer(L); }

@@ -25,6 +25,7 @@
  */
 #include "tl_common.h"
 #include "tl_internal.h"
+#include "tl_chunk.h"
 #include "../../include/tlkv.h"
 
 #include <string.h>
@@ -565,3 +566,6 @@ extern "C" int tl_attn_decode_batch_q8(const tl_decode_seq_q8 *seqs, uint32_t n_
     return tl_launch_decode(p, n_seq, L0->head_dim, n_head / L0->n_kv_head, max_vis,
                             (hipStream_t)stream, true);
 }
+
+int tl_check_layer_q8(const tl_kv_layer_q8 *L) { return check_layer_q8(L); }
+LayerView tl_view_q8(const tl_kv_layer_q8 *L) { return view_q8(L); }

@@ -49,6 +49,33 @@ MAX_BATCH_SEQ = 16
 class RopeParams(ctypes.Structure):
     _fields_ = [("rope_dim", u32), ("theta", ctypes.c_float), ("neox", ctypes.c_int32)]
 
+
+
+class Chunk(ctypes.Structure):
+    _fields_ = [("pages", vp), ("pos", u32), ("n", u32), ("row", u32), ("prefix", u32),
+                ("rope_skip", u32), ("pad_", u32), ("weight", vp)]
+
+
+class QkNormArgs(ctypes.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("q_weight", vp), ("k_weight", vp),
+                ("eps", ctypes.c_float), ("rows", u32), ("n_head", u32), ("q_stride", u32),
+                ("kv_stride", u32), ("q_out_stride", u32), ("page_size", u32),
+                ("rope", RopeParams)]
+
+
+class ChunkAttnArgs(ctypes.Structure):
+    _fields_ = [("q", vp), ("dst", vp), ("lse", vp), ("first", vp), ("slopes", vp), ("rows", u32),
+                ("n_head", u32), ("q_stride", u32), ("page_size", u32), ("window", u32),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("ws", vp),
+                ("ws_bytes", ctypes.c_uint64)]
+
+
+class EvictSeq(ctypes.Structure):
+    _fields_ = [("weight", vp), ("pages", vp), ("len", u32), ("keep", u32), ("sink", u32),
+                ("recent", u32), ("page_size", u32), ("pad_", u32), ("kept", vp), ("rows", vp),
+                ("freed", vp), ("weight_out", vp)]
+
+
 _lib = None
 
 
@@ -141,6 +168,21 @@ def lib():
                             ctypes.POINTER(RopeParams), vp],
         "tl_kv_append_rope_q8": [ctypes.POINTER(KvLayerQ8), vp, vp, u32, vp, u32, u32,
                                  ctypes.POINTER(RopeParams), vp],
+        "tl_qk_norm_append": [ctypes.POINTER(KvLayer), ctypes.POINTER(QkNormArgs),
+                              ctypes.POINTER(Chunk), u32, vp],
+        "tl_qk_norm_append_q8": [ctypes.POINTER(KvLayerQ8), ctypes.POINTER(QkNormArgs),
+                                 ctypes.POINTER(Chunk), u32, vp],
+        "tl_attn_chunks": [ctypes.POINTER(KvLayer), ctypes.POINTER(ChunkAttnArgs),
+                           ctypes.POINTER(Chunk), u32, vp],
+        "tl_attn_chunks_q8": [ctypes.POINTER(KvLayerQ8), ctypes.POINTER(ChunkAttnArgs),
+                              ctypes.POINTER(Chunk), u32, vp],
+        "tl_attn_chunks_ws": [u32, u32, ctypes.POINTER(ChunkAttnArgs), ctypes.POINTER(Chunk), u32,
+                              ctypes.POINTER(ctypes.c_uint64)],
+        "tl_attn_weight": [ctypes.POINTER(KvLayer), ctypes.POINTER(ChunkAttnArgs),
+                           ctypes.POINTER(Chunk), u32, vp],
+        "tl_attn_weight_q8": [ctypes.POINTER(KvLayerQ8), ctypes.POINTER(ChunkAttnArgs),
+                              ctypes.POINTER(Chunk), u32, vp],
+        "tl_kv_evict": [ctypes.POINTER(EvictSeq), u32, vp],
     }
     for name, args in sigs.items():
         f = getattr(L, name)
