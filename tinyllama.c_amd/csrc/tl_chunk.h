@@ -7,7 +7,8 @@
 #define CK_MAX_SEQ 32          /* chunks of one launch; longer batches take several */
 #define CK_MAX_CHUNKS 4096     /* chunks of one call */
 #define CK_KEYS 32             /* keys of one tile */
-#define CK_COLS 16             /* (row, head) columns of one narrow tile */
+#define CK_COLS 16             /* (row, head) columns of a narrow workgroup */
+#define CK_WCOLS 128           /* ... of a wide one */
 
 /* Split merge: one arrival counter per group, zero between launches, at the
  * start of the workspace; (max, sum) pairs and partial rows follow. */
@@ -18,12 +19,12 @@ static_assert(CK_CNT_WORDS <= TL_MERGE_CNT_WORDS, "counters of a stream's worksp
 
 /* One chunk of a launch: its workgroups are [wg0, next wg0), ncb column blocks
  * x n_kv heads x ns key splits of them; part0 / grp0: its first partial row
- * set and merge counter (ns > 1). */
+ * and merge counter (ns > 1). */
 struct CkSeq {
     const u32 *pages;
     float *weight;
     u32 pos, n, row, prefix, rope_skip;
-    u32 wg0, ncb, ns, part0, grp0;
+    u32 wg0, ncb, ns, part0, grp0;   /* part0 counts columns */
 };
 
 struct CkCache {
@@ -140,39 +141,51 @@ TL_DEV u32 group_umax(u32 x) {
 }
 TL_DEV u32 ck_uniform(u32 x) { return (u32)__builtin_amdgcn_readfirstlane((int)x); }
 
-/* The key tiles that a block of columns needs: [a0, a0 + na) of the prefix,
- * then nb from b0 on.  full(): every column sees every key of a tile. */
-struct CkTiles {
-    u32 a0, na, b0, nb;
-    u32 max_lo, min_hi, max_f, pre;
+/* What a block of columns sees together: the lowest and highest keys of its
+ * causal part and of its prefix, and the range that every column sees. */
+struct CkSpan {
+    u32 fmin, lo, hi, max_lo, min_hi, max_f, pre;
     /* N: lanes over which the columns lie (the other lanes repeat them) */
     template <int N>
     TL_DEV void set(const CkSees &s) {
-        const u32 none = 0xffffffffu;
-        const u32 fmin = ck_uniform(group_umin<N>(s.pw ? s.f : none));
-        const u32 lo = ck_uniform(group_umin<N>(s.w ? s.lo : none));
-        const u32 hi = ck_uniform(group_umax<N>(s.w ? s.hi : 0));
+        fmin = ck_uniform(group_umin<N>(s.pw ? s.f : ~0u));
+        lo = ck_uniform(group_umin<N>(s.w ? s.lo : ~0u));
+        hi = ck_uniform(group_umax<N>(s.w ? s.hi : 0));
         max_lo = ck_uniform(group_umax<N>(s.lo));
         min_hi = ck_uniform(group_umin<N>(s.hi));
         max_f = ck_uniform(group_umax<N>(s.f));
         pre = ck_uniform(s.pre);
+    }
+    /* every column sees every one of the n keys from kb on */
+    TL_DEV bool full(u32 kb, u32 n) const {
+        return (kb >= max_lo && kb + n <= min_hi) || (kb >= max_f && kb + n <= pre);
+    }
+    /* some column may see one of them */
+    TL_DEV bool any(u32 kb, u32 n) const {
+        return (kb < hi && kb + n > lo) || (kb < pre && kb + n > fmin);
+    }
+};
+
+/* The tiles of KT keys that they need: na from a0 on of the prefix, then nb
+ * from b0 on. */
+template <u32 KT>
+struct CkTiles {
+    u32 a0, na, b0, nb;
+    TL_DEV void set(const CkSpan &s) {
         a0 = na = b0 = nb = 0;
-        if (fmin != none) {
-            a0 = fmin / CK_KEYS;
-            na = (pre + CK_KEYS - 1) / CK_KEYS - a0;
+        if (s.fmin != ~0u) {
+            a0 = s.fmin / KT;
+            na = (s.pre + KT - 1) / KT - a0;
         }
-        if (lo != none) {
-            b0 = lo / CK_KEYS;
-            u32 b1 = (hi + CK_KEYS - 1) / CK_KEYS;
+        if (s.lo != ~0u) {
+            b0 = s.lo / KT;
+            const u32 b1 = (s.hi + KT - 1) / KT;
             if (na && b0 < a0 + na) b0 = a0 + na;
             nb = b1 > b0 ? b1 - b0 : 0;
         }
     }
     TL_DEV u32 count() const { return na + nb; }
-    TL_DEV u32 key(u32 t) const { return (t < na ? a0 + t : b0 + (t - na)) * CK_KEYS; }
-    TL_DEV bool full(u32 kb) const {
-        return (kb >= max_lo && kb + CK_KEYS <= min_hi) || (kb >= max_f && kb + CK_KEYS <= pre);
-    }
+    TL_DEV u32 key(u32 t) const { return (t < na ? a0 + t : b0 + (t - na)) * KT; }
 };
 
 /* ---- one wave's tile of 32 keys x 16 columns, operands straight from memory --
@@ -341,26 +354,29 @@ template <int D>
 struct CkTile<D, true> : CkTileQ8<D> {};
 
 /* q of a column as f16 pairs, scaled by its row's power of two; returns the
- * factor that takes the products back to scale * q.k */
-template <int D>
-TL_DEV float ck_load_q(const float *qrow, u32 g, float scale, h8_t (&hi)[D / 32], h8_t (&lo)[D / 32]) {
-    float x[D / 32][8];
+ * factor that takes the products back to scale * q.k.  The column's row lies
+ * over G lanes, 64 / G apart: lane g of them holds dims 8 (G s + g) .. of step s */
+template <int D, int G>
+TL_DEV float ck_load_q(const float *qrow, u32 g, float scale, h8_t (&hi)[D / (8 * G)],
+                       h8_t (&lo)[D / (8 * G)]) {
+    constexpr int N = D / (8 * G);
+    float x[N][8];
     float m = 0.f;
 #pragma unroll
-    for (int s = 0; s < D / 32; s++) {
-        const float4 a = *(const float4 *)(qrow + 32 * s + 8 * g);
-        const float4 b = *(const float4 *)(qrow + 32 * s + 8 * g + 4);
+    for (int s = 0; s < N; s++) {
+        const float4 a = *(const float4 *)(qrow + 8 * (G * s + g));
+        const float4 b = *(const float4 *)(qrow + 8 * (G * s + g) + 4);
         x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
         x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
         m = fmaxf(m, amax8(x[s]));
     }
-    m = fmaxf(m, __shfl_xor(m, 16));
+    if constexpr (G == 4) m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     const int e = ck_row_exp(m);
     const float up = __uint_as_float((u32)(e + 127) << 23);
     const float down = __uint_as_float((u32)(127 - e) << 23);
 #pragma unroll
-    for (int s = 0; s < D / 32; s++)
+    for (int s = 0; s < N; s++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             _Float16 h, l;

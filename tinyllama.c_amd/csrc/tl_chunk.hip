@@ -324,47 +324,64 @@ static u64 span_tiles(const tl_chunk &c, u32 window, u32 r0, u32 r1) {
     return (pre + CK_KEYS - 1) / CK_KEYS + (hi > lo ? (hi + CK_KEYS - 1) / CK_KEYS - lo / CK_KEYS : 0);
 }
 
+/* One launch of the narrow kernel and one of the wide, and their workspace. */
 struct AttnPlan {
-    u32 wgs;           /* workgroups of the launch */
-    u64 sets;          /* partial sets of 16 rows */
-    u32 groups;        /* merge counters */
+    CkSeq seq[2][CK_MAX_SEQ];   /* [0]: narrow, [1]: wide */
+    u32 n[2], wgs[2];
+    u64 parts;                  /* partial rows */
+    u32 groups;                 /* merge counters (narrow) */
 };
 
-/* Workgroups of ck_wave tiles: as many splits as fill the chip twice over (two
- * workgroups to a CU), none of fewer than one tile for each wave. */
-static AttnPlan plan_attn(CkSeq *seq, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 window) {
-    u64 total = 0;
-    u64 tiles[CK_MAX_SEQ];
+/* More columns than this take the wide kernel. */
+#define CK_WIDE_MIN 32
+
+/* As many splits as fill the chip with two workgroups to a CU (one at
+ * head_dim 256), none of fewer keys than 128 (one tile for each narrow wave) or
+ * 256 (wide: partial rows of 128 columns cost more to join). */
+static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
+                      u32 window) {
+    pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
+    pl.parts = 0;
+    u64 tiles[2][CK_MAX_SEQ], total[2] = {0, 0};
     for (u32 i = 0; i < n; i++) {
-        seq[i].ncb = (u32)(((u64)seq[i].n * gqa + CK_COLS - 1) / CK_COLS);
-        tiles[i] = span_tiles(*ch[i], window, 0, ch[i]->n);
-        total += tiles[i] * seq[i].ncb * n_kv;
+        const u64 cols = (u64)ch[i]->n * gqa;
+        const int w = cols > CK_WIDE_MIN;
+        CkSeq &s = pl.seq[w][pl.n[w]];
+        seq_of(s, *ch[i]);
+        const u32 per = w ? CK_WCOLS : CK_COLS;
+        s.ncb = (u32)((cols + per - 1) / per);
+        tiles[w][pl.n[w]++] = span_tiles(*ch[i], window, 0, ch[i]->n);
+        total[w] += tiles[w][pl.n[w] - 1] * s.ncb * n_kv;
     }
-    u64 per = (total + 511) / 512;
-    if (per < 4) per = 4;
-    AttnPlan pl = {0, 0, 0};
-    u64 wgs = 0;
-    for (u32 i = 0; i < n; i++) {
-        u64 ns = (tiles[i] + per - 1) / per;
-        const u64 groups = (u64)seq[i].ncb * n_kv;
-        if (ns < 1 || pl.groups + groups > CK_MAX_GROUPS) ns = 1;
-        seq[i].ns = (u32)ns;
-        seq[i].wg0 = (u32)wgs;
-        seq[i].part0 = (u32)pl.sets;
-        seq[i].grp0 = pl.groups;
-        wgs += groups * ns;
-        if (ns > 1) {
-            pl.sets += groups * ns;
-            pl.groups += (u32)groups;
+    const u32 fill = head_dim == 256 ? 256 : 512;
+    for (int w = 0; w < 2; w++) {
+        u64 per = (total[w] + fill - 1) / fill, wgs = 0;
+        const u64 least = w ? 8 : 4;
+        if (per < least) per = least;
+        for (u32 i = 0; i < pl.n[w]; i++) {
+            CkSeq &s = pl.seq[w][i];
+            u64 ns = (tiles[w][i] + per - 1) / per;
+            const u64 groups = (u64)s.ncb * n_kv;
+            if (ns < 1 || (!w && pl.groups + groups > CK_MAX_GROUPS)) ns = 1;
+            s.ns = (u32)ns;
+            s.wg0 = (u32)wgs;
+            s.part0 = (u32)pl.parts;
+            s.grp0 = pl.groups;
+            wgs += groups * ns;
+            if (ns > 1) {
+                pl.parts += groups * ns * (w ? CK_WCOLS : CK_COLS);
+                if (!w) pl.groups += (u32)groups;
+            }
         }
+        if (wgs > 0x7fffffffull || pl.parts > 0xffffffffull) return false;
+        pl.wgs[w] = (u32)wgs;
     }
-    pl.wgs = wgs > 0x7fffffffull ? 0 : (u32)wgs;
-    return pl;
+    return true;
 }
 
 #define CK_WS_HEAD ((u64)CK_CNT_WORDS * sizeof(u32))
-static u64 ws_need(u64 sets, u32 head_dim) {
-    return CK_WS_HEAD + sets * CK_COLS * (sizeof(float2) + (u64)head_dim * sizeof(float));
+static u64 ws_need(u64 parts, u32 head_dim) {
+    return CK_WS_HEAD + parts * (sizeof(float2) + (u64)head_dim * sizeof(float));
 }
 
 static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
@@ -386,28 +403,26 @@ static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_
 }
 
 /* the call's chunks with rows, at most CK_MAX_SEQ of them from *at on */
-static u32 next_chunks(const tl_chunk *ch, u32 n_chunk, u32 *at, CkSeq *seq, const tl_chunk **of) {
+static u32 next_chunks(const tl_chunk *ch, u32 n_chunk, u32 *at, const tl_chunk **of) {
     u32 m = 0;
     for (; *at < n_chunk && m < CK_MAX_SEQ; (*at)++)
-        if (ch[*at].n) {
-            seq_of(seq[m], ch[*at]);
-            of[m++] = &ch[*at];
-        }
+        if (ch[*at].n) of[m++] = &ch[*at];
     return m;
 }
 
-/* most partial sets that a launch of the call takes */
-static u64 most_sets(u32 n_kv, u32 gqa, u32 window, const tl_chunk *ch, u32 n_chunk) {
-    CkSeq seq[CK_MAX_SEQ];
+/* most partial rows that the launches of one group of chunks take */
+static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, u32 window, const tl_chunk *ch, u32 n_chunk,
+                       u64 *parts) {
+    AttnPlan pl;
     const tl_chunk *of[CK_MAX_SEQ];
-    u64 most = 0;
+    *parts = 0;
     for (u32 i = 0; i < n_chunk;) {
-        const u32 m = next_chunks(ch, n_chunk, &i, seq, of);
+        const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        const AttnPlan pl = plan_attn(seq, of, m, n_kv, gqa, window);
-        most = pl.sets > most ? pl.sets : most;
+        if (!plan_attn(pl, of, m, n_kv, gqa, head_dim, window)) return false;
+        *parts = pl.parts > *parts ? pl.parts : *parts;
     }
-    return most;
+    return true;
 }
 
 extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl_chunk_attn_args *a,
@@ -415,24 +430,25 @@ extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl
     if (!a || !bytes || (n_chunk && !chunks) || n_chunk > CK_MAX_CHUNKS || !n_kv_head || !a->n_head ||
         a->n_head % n_kv_head || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return tl_fail(TL_EINVAL, "attn_chunks_ws: arguments");
-    *bytes = ws_need(most_sets(n_kv_head, a->n_head / n_kv_head, a->window, chunks, n_chunk), head_dim);
+    u64 parts;
+    if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, a->window, chunks, n_chunk, &parts))
+        return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
+    *bytes = ws_need(parts, head_dim);
     return TL_OK;
 }
 
 /* where the call's counters, pairs and partial rows lie (its launches take
  * them one after another) */
-static int take_ws(const tl_chunk_attn_args *a, u64 sets, u32 head_dim, hipStream_t st, CkAttnParams &p) {
-    if (!sets) return TL_OK;
-    if (sets * CK_COLS * head_dim * sizeof(float) > 0x7ffffff0ull)
-        return tl_fail(TL_ERANGE, "attn_chunks: %llu partial sets", (unsigned long long)sets);
+static int take_ws(const tl_chunk_attn_args *a, u64 parts, u32 head_dim, hipStream_t st, CkAttnParams &p) {
+    if (!parts) return TL_OK;
     if (a->ws) {
-        const u64 need = ws_need(sets, head_dim);
+        const u64 need = ws_need(parts, head_dim);
         if (a->ws_bytes < need)
             return tl_fail(TL_ERANGE, "attn_chunks: workspace of %llu bytes, %llu needed",
                            (unsigned long long)a->ws_bytes, (unsigned long long)need);
         p.cnt = (u32 *)a->ws;
         p.ws_ml = (float2 *)((char *)a->ws + CK_WS_HEAD);
-        p.ws_acc = (float *)(p.ws_ml + sets * CK_COLS);
+        p.ws_acc = (float *)(p.ws_ml + parts);
         return TL_OK;
     }
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -440,7 +456,7 @@ static int take_ws(const tl_chunk_attn_args *a, u64 sets, u32 head_dim, hipStrea
     if (cs != hipStreamCaptureStatusNone)
         return tl_fail(TL_EINVAL, "attn_chunks: a captured call takes its own workspace (ws)");
     TlWorkspace *w;
-    const int rc = tl_workspace_get(st, sets * CK_COLS * head_dim, sets * CK_COLS, TL_MERGE_CNT_WORDS, &w);
+    const int rc = tl_workspace_get(st, parts * head_dim, parts, TL_MERGE_CNT_WORDS, &w);
     if (rc) return rc;
     p.cnt = w->cnt;
     p.ws_ml = (float2 *)w->ml;
@@ -474,17 +490,40 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
         return tl_fail(TL_EINVAL, "attn_chunks: dst overlaps q");
     CkAttnParams p;
     fill_attn(p, L, a, shift);
-    rc = take_ws(a, most_sets(L.n_kv_head, p.gqa, a->window, ch, n_chunk), L.head_dim, st, p);
+    u64 parts;
+    if (!most_parts(L.n_kv_head, p.gqa, L.head_dim, a->window, ch, n_chunk, &parts))
+        return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
+    rc = take_ws(a, parts, L.head_dim, st, p);
     if (rc) return rc;
     const tl_chunk *of[CK_MAX_SEQ];
+    AttnPlan pl;
     for (u32 i = 0; i < n_chunk;) {
-        const u32 m = next_chunks(ch, n_chunk, &i, p.seq, of);
+        const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        p.n_seq = m;
-        const AttnPlan pl = plan_attn(p.seq, of, m, L.n_kv_head, p.gqa, a->window);
-        if (!pl.wgs) return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
-        ck_launch_attn(p, L.head_dim, L.q8, pl.wgs, st);
-        HIP_TRY(hipGetLastError());
+        plan_attn(pl, of, m, L.n_kv_head, p.gqa, L.head_dim, a->window);
+        for (int w = 1; w >= 0; w--) {
+            if (!pl.wgs[w]) continue;
+            p.n_seq = pl.n[w];
+            memcpy(p.seq, pl.seq[w], pl.n[w] * sizeof(CkSeq));
+            if (w) ck_launch_wide(p, L.head_dim, L.q8, pl.wgs[w], st);
+            else ck_launch_attn(p, L.head_dim, L.q8, pl.wgs[w], st);
+            HIP_TRY(hipGetLastError());
+            if (!w) continue;
+            /* the wide chunks with several splits are joined */
+            u32 k = 0;
+            u64 blocks = 0;
+            const u32 per = 1024 / L.head_dim;      /* columns of a block */
+            for (u32 j = 0; j < pl.n[1]; j++)
+                if (pl.seq[1][j].ns > 1) {
+                    p.seq[k] = pl.seq[1][j];
+                    p.seq[k++].wg0 = (u32)blocks;
+                    blocks += ((u64)pl.seq[1][j].n * p.gqa * L.n_kv_head + per - 1) / per;
+                }
+            if (!k) continue;
+            p.n_seq = k;
+            ck_launch_merge(p, L.head_dim, (u32)blocks, st);
+            HIP_TRY(hipGetLastError());
+        }
     }
     return TL_OK;
 }
@@ -521,11 +560,12 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
     fill_attn(p, L, a, shift);
     const tl_chunk *of[CK_MAX_SEQ];
     for (u32 i = 0; i < n_chunk;) {
-        const u32 m = next_chunks(ch, n_chunk, &i, p.seq, of);
+        const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
         p.n_seq = m;
         u64 wgs = 0;
         for (u32 j = 0; j < m; j++) {
+            seq_of(p.seq[j], *of[j]);
             p.seq[j].wg0 = (u32)wgs;
             p.seq[j].ncb = (u32)(((u64)p.seq[j].n * p.gqa + CK_COLS - 1) / CK_COLS);
             wgs += ((u64)p.seq[j].pos + p.seq[j].n + CK_KEYS - 1) / CK_KEYS;
@@ -557,6 +597,12 @@ void ck_launch_attn(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipSt
     if (head_dim == 64) q8 ? ck_launch_attn_t<64, true>(p, wgs, st) : ck_launch_attn_t<64, false>(p, wgs, st);
     else if (head_dim == 128) q8 ? ck_launch_attn_t<128, true>(p, wgs, st) : ck_launch_attn_t<128, false>(p, wgs, st);
     else q8 ? ck_launch_attn_t<256, true>(p, wgs, st) : ck_launch_attn_t<256, false>(p, wgs, st);
+}
+
+void ck_launch_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) q8 ? ck_launch_wide_t<64, true>(p, wgs, st) : ck_launch_wide_t<64, false>(p, wgs, st);
+    else if (head_dim == 128) q8 ? ck_launch_wide_t<128, true>(p, wgs, st) : ck_launch_wide_t<128, false>(p, wgs, st);
+    else q8 ? ck_launch_wide_t<256, true>(p, wgs, st) : ck_launch_wide_t<256, false>(p, wgs, st);
 }
 
 void ck_launch_weight(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {

@@ -11,6 +11,13 @@ void ck_launch_attn_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
         hipLaunchKernelGGL((chunk_attn_kernel<D, Q8, false>), dim3(wgs), dim3(64 * CK_WAVES), 0, st, p);
 }
 template <int D, bool Q8>
+void ck_launch_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
+    if (p.softcap > 0.f || p.slopes)
+        hipLaunchKernelGGL((chunk_attn_wide_kernel<D, Q8, true>), dim3(wgs), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((chunk_attn_wide_kernel<D, Q8, false>), dim3(wgs), dim3(256), 0, st, p);
+}
+template <int D, bool Q8>
 void ck_launch_weight_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
     if (p.softcap > 0.f || p.slopes)
         hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, true>), dim3(wgs), dim3(256), 0, st, p);
@@ -23,3 +30,12 @@ template void ck_launch_attn_t<256, false>(const CkAttnParams &, u32, hipStream_
 template void ck_launch_weight_t<64, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_weight_t<128, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_weight_t<256, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_wide_t<64, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_wide_t<128, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_wide_t<256, false>(const CkAttnParams &, u32, hipStream_t);
+
+void ck_launch_merge(const CkAttnParams &p, u32 head_dim, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) hipLaunchKernelGGL(chunk_merge_kernel<64>, dim3(wgs), dim3(256), 0, st, p);
+    else if (head_dim == 128) hipLaunchKernelGGL(chunk_merge_kernel<128>, dim3(wgs), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(chunk_merge_kernel<256>, dim3(wgs), dim3(256), 0, st, p);
+}

@@ -36,15 +36,17 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     const u64 brow = (u64)sq.row + r;
 
     h8_t qh[KS], ql[KS];
-    float cs = ck_load_q<D>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
+    float cs = ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
     if constexpr (!BIAS) cs *= CK_LOG2E;
     const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
     const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
 
     CkSees see;
     see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
-    CkTiles tiles;
-    tiles.set<16>(see);
+    CkSpan span;
+    span.set<16>(see);
+    CkTiles<CK_KEYS> tiles;
+    tiles.set(span);
     const u32 n_tiles = tiles.count();
     const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
 
@@ -106,21 +108,24 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             rows_k(rn, rk);
             tile.load_k(p.c, kvh, rk, g);
         }
-        u64 seen[8];
-        bool slow = false;
-        const bool full = tiles.full(kb) && !bad;
-        if (!full) {
-            bool odd = false;
+        if (!span.full(kb, CK_KEYS) || bad) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const bool vis = see.sees(kb + 8 * g + e) && !((bad >> (8 * g + e)) & 1);
                 x[e] = vis ? x[e] : -INFINITY;
-                seen[e] = __ballot(vis);
-                const u32 mine = (u32)(seen[e] >> (16 * g)) & 0xffffu;
-                if (mine == 0) tile.clear_v(e);
-                else if (mine != 0xffffu) odd |= tile.odd_v(e);
+                const u32 mine = (u32)(__ballot(vis) >> (16 * g)) & 0xffffu;
+                if (mine == 0) {
+                    tile.clear_v(e);
+                } else if (__any(mine != 0xffffu)) {
+                    /* seen by some columns: infinities and NaN go to those alone */
+                    const bool odd = mine != 0xffffu && tile.odd_v(e);
+                    const u64 ob = __ballot(odd);
+                    if (ob) {
+                        if (odd) tile.clear_v(e);
+                        if (vis && ((ob >> (16 * g)) & 0xffffu)) l = NAN;
+                    }
+                }
             }
-            slow = __any(odd);
         }
         /* running maximum */
         float top = x[0];
@@ -148,33 +153,13 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             ph[e] = a;
             pl[e] = b;
         }
-        if (!slow) {
 #pragma unroll
-            for (int j = 0; j < NM; j++) {
-                h8_t vh, vl;
-                tile.get_v(j, vh, vl);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[j], 0, 0, 0);
-                if constexpr (Q8) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[j], 0, 0, 0);
-            }
-        } else {
-            /* a key that only some columns see holds infinities or NaN: column
-             * by column, the others' keys as zeros */
-            for (u32 c = 0; c < CK_COLS; c++) {
-                CkTile<D, Q8> tc = tile;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (!((seen[e] >> (16 * g + c)) & 1)) tc.clear_v(e);
-#pragma unroll
-                for (int j = 0; j < NM; j++) {
-                    h8_t vh, vl;
-                    tc.get_v(j, vh, vl);
-                    f4_t s = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[j], 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, s, 0, 0, 0);
-                    if constexpr (Q8) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, s, 0, 0, 0);
-                    if (i == c) o[j] = s;
-                }
-            }
+        for (int j = 0; j < NM; j++) {
+            h8_t vh, vl;
+            tile.get_v(j, vh, vl);
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[j], 0, 0, 0);
+            o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[j], 0, 0, 0);
+            if constexpr (Q8) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, o[j], 0, 0, 0);
         }
         if (more) {
             u32 rv[8];
@@ -202,9 +187,9 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     constexpr u32 V4 = D / 4;
     const u32 units = ncol * V4;
     const u32 group = kvh * sq.ncb + cb;
-    const u64 set0 = (u64)sq.part0 + (u64)group * sq.ns;      /* the group's first partial set */
-    const __amdgpu_buffer_rsrc_t ra = buf_rsrc(p.ws_acc + set0 * CK_COLS * D);
-    const __amdgpu_buffer_rsrc_t rm = buf_rsrc(p.ws_ml + set0 * CK_COLS);
+    const u64 part = (u64)sq.part0 + (u64)group * sq.ns * CK_COLS;      /* the group's first partial row */
+    const __amdgpu_buffer_rsrc_t ra = buf_rsrc(p.ws_acc + part * D);
+    const __amdgpu_buffer_rsrc_t rm = buf_rsrc(p.ws_ml + part);
     for (u32 u = threadIdx.x; u < units; u += 64 * CK_WAVES) {
         const u32 c = u / V4, d = u % V4;
         float M = -INFINITY;
@@ -230,7 +215,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
                 make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
             if (p.lse && d == 0)
-                p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __log2f(sum)) * CK_LN2;
+                p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
         } else {
             const u32x4v_t v = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(a.z), __float_as_uint(a.w)};
             __builtin_amdgcn_raw_buffer_store_b128(v, ra, ((split * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
@@ -293,8 +278,425 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
         *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
             make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
         if (p.lse && d == 0)
-            p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __log2f(sum)) * CK_LN2;
+            p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
     }
     if (threadIdx.x == 0)
         __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+/* ---- many columns: 128 to a workgroup, K and V tiles shared through LDS ------
+ *
+ * Each of the four waves has 32 columns and runs S^T = K . Q^T and O^T += V^T .
+ * P^T on v_mfma_f32_32x32x16_f16 (A rows: lane & 31, eight k's of half h = lane
+ * >> 5).  A lane's sixteen scores of a 32-key block are rows (r & 3) + 8 (r >>
+ * 2) + 4 h; matrix row rho is fed key rho with bits 2 and 3 exchanged, so they
+ * are keys 16 u + 8 h + j (r = 8 u + j), the k order of step u of the second
+ * product.  Waves 0 and 1 fetch a tile's K rows, waves 2 and 3 its V rows, eight
+ * keys to a lane, which they transpose on the way to LDS (v_perm on pairs), so
+ * that both operands are 16-byte reads.  Units of 16 bytes are permuted within a
+ * row so that 16 lanes' reads cover all banks.  Two buffers, one barrier per
+ * tile; a tile's rows are looked up two tiles ahead, its data fetched one ahead.
+ * A Q8_0 tile is kept as two planes, hi and lo. */
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+template <int D, bool Q8>
+struct CkWide {
+    static constexpr int KT = Q8 ? (D == 64 ? 64 : 32) : (D == 256 ? 32 : 64);
+    static constexpr int U = D / 8;                  /* 16-byte units of a K row in LDS */
+    static constexpr int VU = KT / 8;                /* ... of a V^T row */
+    static constexpr int PL = Q8 ? 2 : 1;
+    static constexpr int DPL = KT * D / 1024;        /* dims of V of a staging lane */
+    static constexpr int RU = Q8 ? D / 16 : D / 8;   /* 16-byte units of a K row in memory */
+    static constexpr int KL = KT * RU / 128;         /* ... of a staging lane */
+    static constexpr int VD = Q8 ? DPL / 4 : DPL / 2;   /* dwords of V of a key and staging lane */
+    static constexpr int ST = KL * 4 > 8 * VD ? KL * 4 : 8 * VD;
+    static constexpr int SC = Q8 ? 8 : 1;            /* scales of a staging lane */
+    static_assert(DPL == 4 || DPL == 8, "staging");
+    static constexpr int KP = KT * U * 16, VP = D * VU * 16;   /* bytes of a plane */
+    /* byte offsets of units; exclusive-or linear in the bits of their arguments, so
+     * an offset is the lane's part with a constant part put in (put) */
+    static constexpr TL_HOSTDEV u32 kat(u32 key, u32 unit) {
+        return (key * U + (unit ^ (U == 8 ? (key >> 1) & 7 : key & 15))) * 16;
+    }
+    static constexpr TL_HOSTDEV u32 vat(u32 dim, u32 unit) {
+        return (dim * VU + (unit ^ (VU == 8 ? ((dim >> 1) ^ (dim >> 3)) & 7 : (dim >> 2) & 3))) * 16;
+    }
+    static TL_DEV u32 kput(u32 lane_part, u32 c) {
+        return (lane_part ^ (c & (U * 16 - 1))) + (c & ~(u32)(U * 16 - 1));
+    }
+    static TL_DEV u32 vput(u32 lane_part, u32 c) {
+        return (lane_part ^ (c & (VU * 16 - 1))) + (c & ~(u32)(VU * 16 - 1));
+    }
+};
+
+template <int D, bool Q8, bool BIAS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
+    typedef CkWide<D, Q8> W;
+    constexpr int KT = W::KT, NS = D / 16, NO = D / 32;
+    /* buffer b, plane l of K: s_k + (b * PL + l) * KP; of V the same */
+    __shared__ __align__(16) char s_k[2 * W::PL * W::KP];
+    __shared__ __align__(16) char s_v[2 * W::PL * W::VP];
+    __shared__ CkSpan s_span[4];
+    __shared__ u64 s_odd[2][2];      /* keys of a tile whose V is not all finite */
+    const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
+    const u32 i = lane & 31, h = lane >> 5;
+    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const u32 local = blockIdx.x - sq.wg0;
+    const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
+    const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
+    const u32 cols = sq.n * p.gqa, cw = cb * CK_WCOLS + wave * 32;
+    const bool live = cw < cols;
+    const u32 col = min(cw + i, cols - 1);
+    const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+    const u32 pq = sq.pos + r, end = sq.pos + sq.n;
+    const u64 brow = (u64)sq.row + r;
+
+    h8_t qh[NS], ql[NS];
+    float cs = ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, p.scale, qh, ql);
+    if constexpr (!BIAS) cs *= CK_LOG2E;
+    const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
+    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+
+    CkSees see;
+    see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
+    CkSpan span, all;
+    span.set<32>(see);
+    if (lane == 0) s_span[wave] = span;
+    __syncthreads();
+    all = s_span[0];
+#pragma unroll
+    for (int w = 1; w < 4; w++) {
+        const CkSpan &o = s_span[w];
+        all.fmin = min(all.fmin, o.fmin);
+        all.lo = min(all.lo, o.lo);
+        all.hi = max(all.hi, o.hi);
+        all.max_lo = max(all.max_lo, o.max_lo);
+        all.min_hi = min(all.min_hi, o.min_hi);
+        all.max_f = max(all.max_f, o.max_f);
+    }
+    CkTiles<KT> tiles;
+    tiles.set(all);
+    tiles.a0 = ck_uniform(tiles.a0);
+    tiles.na = ck_uniform(tiles.na);
+    tiles.b0 = ck_uniform(tiles.b0);
+    tiles.nb = ck_uniform(tiles.nb);
+    const u32 n_tiles = tiles.count();
+    const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
+
+    float m = -INFINITY, l = 0.f;
+    f16_t o[NO];
+#pragma unroll
+    for (int b = 0; b < NO; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[b][e] = 0.f;
+
+    /* staging */
+    u32 st[W::ST];
+    u32 sc[W::SC];
+    const u32 sl = (wave & 1) * 64 + lane;
+    const u32 dg = sl % (D / W::DPL), kg = sl / (D / W::DPL);      /* V: dims and keys of the lane */
+    const char *kbase = (const char *)p.c.k + (u64)kvh * p.c.cap * (Q8 ? D : 2 * D);
+    const char *vbase = (const char *)p.c.v + (u64)kvh * p.c.cap * (Q8 ? D : 2 * D);
+    const u16 *ksb = p.c.ks + (u64)kvh * p.c.cap * (D / 32);
+    const u16 *vsb = p.c.vs + (u64)kvh * p.c.cap * (D / 32);
+    const u32 kst = W::kat(sl / W::RU, (Q8 ? 2 : 1) * (sl % W::RU)), vst = W::vat(dg * W::DPL, kg);
+    auto look = [&](u32 t) -> u32 {
+        const u32 key = tiles.key(t) + (lane & (KT - 1));
+        return key < end ? ck_row(p.c, sq.pages, key) : ~0u;
+    };
+    auto fetch = [&](u32 rc) {
+        if (wave < 2) {
+#pragma unroll
+            for (int j = 0; j < W::KL; j++) {
+                const u32 x = j * 128 + sl, key = x / W::RU, u = x % W::RU;
+                const u32 row = __shfl(rc, key);
+                const u4_t v = *(const u4_t *)(kbase + (u64)(row * (u32)(W::RU * 16) + u * 16));
+#pragma unroll
+                for (int d = 0; d < 4; d++) st[4 * j + d] = v[d];
+                if constexpr (Q8) sc[j] = ksb[(u64)(row * (u32)(D / 32) + (u >> 1))];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const u32 row = __shfl(rc, 8 * kg + e);
+                const char *a = vbase + (u64)(row * (u32)(Q8 ? D : 2 * D) + dg * (Q8 ? W::DPL : 2 * W::DPL));
+                if constexpr (W::VD == 1) {
+                    st[e] = *(const u32 *)a;
+                } else if constexpr (W::VD == 2) {
+                    const uint2 v = *(const uint2 *)a;
+                    st[2 * e] = v.x;
+                    st[2 * e + 1] = v.y;
+                } else {
+                    const u4_t v = *(const u4_t *)a;
+#pragma unroll
+                    for (int d = 0; d < 4; d++) st[4 * e + d] = v[d];
+                }
+                if constexpr (Q8) sc[e] = vsb[(u64)(row * (u32)(D / 32) + dg * W::DPL / 32)];
+            }
+        }
+    };
+    /* bad: keys of the tile without a row; check: V may be seen by some columns only */
+    auto store = [&](u32 buf, u64 bad, bool check) {
+        if (wave < 2) {
+#pragma unroll
+            for (int j = 0; j < W::KL; j++) {
+                char *to = s_k + buf * (W::PL * W::KP);
+                const u32 c = W::kat(j * (128 / W::RU), 0);
+                if constexpr (!Q8) {
+                    *(u4_t *)(to + W::kput(kst, c)) = (u4_t){st[4 * j], st[4 * j + 1], st[4 * j + 2], st[4 * j + 3]};
+                } else {
+                    const tl_half2 d2 = __builtin_bit_cast(tl_half2, sc[j] * 0x10001u);
+                    u32 hi[8], lo[8];
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        tl_half2 a, b;
+                        i8x4_to_f16(st[4 * j + d], a, b);
+                        ck_q8_pair(a, d2, hi[2 * d], lo[2 * d]);
+                        ck_q8_pair(b, d2, hi[2 * d + 1], lo[2 * d + 1]);
+                    }
+#pragma unroll
+                    for (int z = 0; z < 2; z++) {
+                        char *at = to + W::kput(kst, c ^ (z * 16));
+                        *(u4_t *)at = (u4_t){hi[4 * z], hi[4 * z + 1], hi[4 * z + 2], hi[4 * z + 3]};
+                        *(u4_t *)(at + (W::PL - 1) * W::KP) = (u4_t){lo[4 * z], lo[4 * z + 1], lo[4 * z + 2], lo[4 * z + 3]};
+                    }
+                }
+            }
+            return;
+        }
+        if (bad) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if ((bad >> (8 * kg + e)) & 1) {
+#pragma unroll
+                    for (int d = 0; d < W::VD; d++) st[W::VD * e + d] = 0;
+                    if constexpr (Q8) sc[e] = 0;
+                }
+        }
+        if (check) {
+            /* infinities and NaN, which only some columns may see: zeros in the
+             * product, and the columns that do see the key are told */
+            u32 odd = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                bool x = false;
+                if constexpr (Q8) {
+                    x = (sc[e] & 0x7fffu) > 0x6006u;
+                    sc[e] = x ? 0 : sc[e];
+                } else {
+#pragma unroll
+                    for (int d = 0; d < W::VD; d++)
+                        x |= (st[W::VD * e + d] & 0x7c00u) == 0x7c00u || (st[W::VD * e + d] & 0x7c000000u) == 0x7c000000u;
+#pragma unroll
+                    for (int d = 0; d < W::VD; d++) st[W::VD * e + d] = x ? 0 : st[W::VD * e + d];
+                }
+                odd |= (u32)x << e;
+            }
+            u64 keys = 0;
+            if (__any(odd)) {
+                keys = (u64)odd << (8 * kg);
+#pragma unroll
+                for (int x = 1; x < 64; x <<= 1) keys |= __shfl_xor(keys, x);
+            }
+            if (lane == 0) s_odd[buf][wave - 2] = keys;
+        }
+#pragma unroll
+        for (int x = 0; x < W::DPL; x++) {
+            u4_t hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (!Q8) {
+                    hi[j] = __builtin_amdgcn_perm(st[W::VD * (2 * j + 1) + (x >> 1)], st[W::VD * 2 * j + (x >> 1)],
+                                                  x & 1 ? 0x07060302u : 0x05040100u);
+                } else {
+                    const u32 sel = 0x0c000c00u | (u32)(x & 3) | ((u32)(4 + (x & 3)) << 16);
+                    const tl_half2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+                    const u32 b = __builtin_amdgcn_perm(st[W::VD * (2 * j + 1) + (x >> 2)], st[W::VD * 2 * j + (x >> 2)], sel);
+                    const tl_half2 v = __builtin_bit_cast(tl_half2, (b ^ 0x00800080u) | 0x64006400u) - bias;
+                    u32 a, c;
+                    ck_q8_pair(v, __builtin_bit_cast(tl_half2, sc[2 * j] | (sc[2 * j + 1] << 16)), a, c);
+                    hi[j] = a;
+                    lo[j] = c;
+                }
+            }
+            char *at = s_v + buf * (W::PL * W::VP) + W::vput(vst, W::vat(x, 0));
+            *(u4_t *)at = hi;
+            if constexpr (Q8) *(u4_t *)(at + (W::PL - 1) * W::VP) = lo;
+        }
+    };
+
+    const u32 krd = W::kat((i & 19) | ((i & 4) << 1) | ((i & 8) >> 1), h), vrd = W::vat(i, h);
+    u32 next = 0;
+    u64 bad = 0;
+    if (t0 < t1) {
+        const u32 row = look(t0);
+        bad = __ballot(row >= p.c.cap);
+        fetch(row < p.c.cap ? row : 0);
+        if (t0 + 1 < t1) next = look(t0 + 1);
+        store(0, bad, bad || !all.full(tiles.key(t0), KT));
+    }
+    for (u32 t = t0; t < t1; t++) {
+        const u32 buf = (t - t0) & 1;
+        const u32 kt = tiles.key(t);
+        const bool more = t + 1 < t1;
+        __syncthreads();
+        u64 nbad = 0;
+        if (more) {
+            nbad = __ballot(next >= p.c.cap);
+            fetch(next < p.c.cap ? next : 0);
+            if (t + 2 < t1) next = look(t + 2);
+        }
+        if (live && span.any(kt, KT)) {
+            const char *const kp = s_k + buf * (W::PL * W::KP), *const vp = s_v + buf * (W::PL * W::VP);
+#pragma unroll
+            for (int sub = 0; sub < KT / 32; sub++) {
+                const u32 kb = kt + 32 * sub;
+                f16_t s;
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    const char *at = kp + W::kput(krd, W::kat(32 * sub, 2 * j));
+                    const h8_t a = *(const h8_t *)at;
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[j], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[j], s, 0, 0, 0);
+                    if constexpr (Q8) {
+                        const h8_t b = *(const h8_t *)(at + (W::PL - 1) * W::KP);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qh[j], s, 0, 0, 0);
+                    }
+                }
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        s[e] = ck_score<true>(s[e], cs, p.softcap, icap, slope, pq, kb + 16 * (e >> 3) + 8 * h + (e & 7));
+                }
+                const u32 mybad = (u32)(bad >> (32 * sub));
+                if (!span.full(kb, 32) || mybad) {
+                    const u32 odd = (u32)((s_odd[buf][0] | s_odd[buf][1]) >> (32 * sub));
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
+                        const bool v = see.sees(kb + k) && !((mybad >> k) & 1);
+                        s[e] = v ? s[e] : -INFINITY;
+                        if (v && ((odd >> k) & 1)) l = NAN;
+                    }
+                }
+                float top = s[0];
+#pragma unroll
+                for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+                if constexpr (!BIAS) top *= cs;
+                const float thr = m == -INFINITY ? -INFINITY : m + CK_LAZY;
+                if (__any(top > thr)) {
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float mn = top > thr ? top : m;
+                    const float al = m == -INFINITY ? (mn == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - mn);
+                    l *= al;
+#pragma unroll
+                    for (int b = 0; b < NO; b++) o[b] *= al;
+                    m = mn;
+                }
+                const float mref = m == -INFINITY ? 0.f : m - CK_UP;
+                h8_t ph[2], pl[2];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float pe = __builtin_amdgcn_exp2f(BIAS ? s[e] - mref : fmaf(s[e], cs, -mref));
+                    l += pe;
+                    _Float16 a, b;
+                    ck_split(pe, a, b);
+                    ph[e >> 3][e & 7] = a;
+                    pl[e >> 3][e & 7] = b;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int b = 0; b < NO; b++) {
+                        const char *at = vp + W::vput(vrd, W::vat(32 * b, 4 * sub + 2 * u));
+                        const h8_t v = *(const h8_t *)at;
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u], o[b], 0, 0, 0);
+                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u], o[b], 0, 0, 0);
+                        if constexpr (Q8) {
+                            const h8_t w = *(const h8_t *)(at + (W::PL - 1) * W::VP);
+                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ph[u], o[b], 0, 0, 0);
+                        }
+                    }
+            }
+        }
+        if (more) store(buf ^ 1, nbad, nbad || !all.full(tiles.key(t + 1), KT));
+        bad = nbad;
+    }
+    l += __shfl_xor(l, 32);
+    if (!live || cw + i >= cols) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (sq.ns == 1) {
+        float *d = p.dst + brow * p.q_stride + (u64)head * D + 4 * h;
+#pragma unroll
+        for (int b = 0; b < NO; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                *(float4 *)(d + 32 * b + 8 * e) = make_float4(o[b][4 * e] * inv, o[b][4 * e + 1] * inv,
+                                                             o[b][4 * e + 2] * inv, o[b][4 * e + 3] * inv);
+        if (p.lse && h == 0)
+            p.lse[brow * p.n_head + head] = l == 0.f ? -INFINITY
+                : ((m == -INFINITY ? 0.f : m) - CK_UP + __builtin_amdgcn_logf(l)) * CK_LN2;
+        return;
+    }
+    const u64 part = (u64)sq.part0 + ((u64)(kvh * sq.ncb + cb) * sq.ns + split) * CK_WCOLS + wave * 32 + i;
+    float *d = p.ws_acc + part * D + 4 * h;
+#pragma unroll
+    for (int b = 0; b < NO; b++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            *(float4 *)(d + 32 * b + 8 * e) = make_float4(o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]);
+    if (h == 0) p.ws_ml[part] = make_float2(m, l);
+}
+
+/* The splits of the wide columns joined: D / 4 threads to a column, a float4
+ * each, eight splits' loads in flight. */
+template <int D>
+__global__ __launch_bounds__(256) void chunk_merge_kernel(const CkAttnParams p) {
+    constexpr u32 V4 = D / 4, CPB = 256 / V4;
+    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const u32 at = (blockIdx.x - sq.wg0) * CPB + threadIdx.x / V4, d = threadIdx.x % V4;
+    const u32 cols = sq.n * p.gqa;
+    const u32 kvh = at / cols, col = at % cols;
+    if (kvh >= p.c.n_kv) return;
+    const u32 cb = col / CK_WCOLS;
+    const u64 part = (u64)sq.part0 + (u64)(kvh * sq.ncb + cb) * sq.ns * CK_WCOLS + col % CK_WCOLS;
+    float M = -INFINITY, sum = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (u32 s0 = 0; s0 < sq.ns; s0 += 8) {
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const u64 x = part + (u64)min(s0 + j, sq.ns - 1) * CK_WCOLS;
+            ml[j] = p.ws_ml[x];
+            v[j] = *(const float4 *)(p.ws_acc + x * D + 4 * d);
+        }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < 8; j++) Mn = fmaxf(Mn, s0 + j < sq.ns ? ml[j].x : -INFINITY);
+        const float M0 = Mn == -INFINITY ? 0.f : Mn;
+        const float f0 = __builtin_amdgcn_exp2f(M - M0);
+        sum *= f0;
+        a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (s0 + j >= sq.ns) break;
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - M0);
+            sum = fmaf(f, ml[j].y, sum);
+            a.x = fmaf(f, v[j].x, a.x);
+            a.y = fmaf(f, v[j].y, a.y);
+            a.z = fmaf(f, v[j].z, a.z);
+            a.w = fmaf(f, v[j].w, a.w);
+        }
+        M = Mn;
+    }
+    const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+    const u64 brow = (u64)sq.row + r;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *(float4 *)(p.dst + brow * p.q_stride + (u64)head * D + 4 * d) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    if (p.lse && d == 0)
+        p.lse[brow * p.n_head + head] = sum == 0.f ? -INFINITY
+            : ((M == -INFINITY ? 0.f : M) - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
 }

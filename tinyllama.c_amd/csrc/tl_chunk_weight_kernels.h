@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
             for (int e = 0; e < 8; e++) any |= see.sees(kb + 8 * g + e);
             if (!__any(any && real)) continue;
             h8_t qh[KS], ql[KS];
-            float cs = ck_load_q<D>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
+            float cs = ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
             if constexpr (!BIAS) cs *= CK_LOG2E;
             const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
             const float lse = p.lse[brow * p.n_head + head] * CK_LOG2E;
