@@ -34,6 +34,7 @@ struct CkCache {
 };
 
 struct CkAttnParams {
+    u32 wg0[CK_MAX_SEQ];       /* seq[].wg0 side by side, ~0 past n_seq */
     CkSeq seq[CK_MAX_SEQ];
     CkCache c;
     const float *q;
@@ -71,11 +72,12 @@ TL_DEV u32 ck_row(const CkCache &c, const u32 *pages, u32 p) {
     return pg <= c.cap >> c.shift ? (pg << c.shift) + (p & ((1u << c.shift) - 1)) : ~0u;
 }
 
-/* index of the launch's chunk that workgroup b belongs to (wg0 rises) */
-TL_DEV u32 ck_find(const CkSeq *seq, u32 n_seq, u32 b) {
-    const u32 lane = threadIdx.x & 63;
-    const bool le = lane < n_seq && seq[lane].wg0 <= b;
-    return (u32)__builtin_amdgcn_readfirstlane((int)__popcll(__ballot(le)) - 1);
+/* index of the launch's chunk that workgroup b belongs to (wg0 rises): one
+ * load of all the starts, one comparison each */
+TL_DEV u32 ck_find(const u32 *wg0, u32 n_seq, u32 b) {
+    if (n_seq == 1) return 0;
+    const u32 lane = threadIdx.x & (CK_MAX_SEQ - 1);
+    return (u32)__builtin_amdgcn_readfirstlane((int)__popc((u32)__ballot(wg0[lane] <= b)) - 1);
 }
 
 /* exp(2|x|) based above 1/4 ((e - 1) / (e + 1): the subtraction is exact to
@@ -355,21 +357,25 @@ struct CkTile<D, true> : CkTileQ8<D> {};
 
 /* q of a column as f16 pairs, scaled by its row's power of two; returns the
  * factor that takes the products back to scale * q.k.  The column's row lies
- * over G lanes, 64 / G apart: lane g of them holds dims 8 (G s + g) .. of step s */
+ * over G lanes, 64 / G apart: lane g of them holds dims 8 (G s + g) .. of step s.
+ * load and split apart, so that other loads can be requested in between. */
 template <int D, int G>
-TL_DEV float ck_load_q(const float *qrow, u32 g, float scale, h8_t (&hi)[D / (8 * G)],
-                       h8_t (&lo)[D / (8 * G)]) {
+TL_DEV void ck_load_q(const float *qrow, u32 g, float4 (&x)[D / (8 * G)][2]) {
+#pragma unroll
+    for (int s = 0; s < D / (8 * G); s++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) x[s][j] = *(const float4 *)(qrow + 8 * (G * s + g) + 4 * j);
+}
+template <int D, int G>
+TL_DEV float ck_split_q(const float4 (&x)[D / (8 * G)][2], float scale, h8_t (&hi)[D / (8 * G)],
+                        h8_t (&lo)[D / (8 * G)]) {
     constexpr int N = D / (8 * G);
-    float x[N][8];
     float m = 0.f;
 #pragma unroll
-    for (int s = 0; s < N; s++) {
-        const float4 a = *(const float4 *)(qrow + 8 * (G * s + g));
-        const float4 b = *(const float4 *)(qrow + 8 * (G * s + g) + 4);
-        x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
-        x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
-        m = fmaxf(m, amax8(x[s]));
-    }
+    for (int s = 0; s < N; s++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(x[s][j].x), fabsf(x[s][j].y))), fmaxf(fabsf(x[s][j].z), fabsf(x[s][j].w)));
     if constexpr (G == 4) m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     const int e = ck_row_exp(m);
@@ -378,11 +384,15 @@ TL_DEV float ck_load_q(const float *qrow, u32 g, float scale, h8_t (&hi)[D / (8 
 #pragma unroll
     for (int s = 0; s < N; s++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            _Float16 h, l;
-            ck_split(x[s][j] * up, h, l);
-            hi[s][j] = h;
-            lo[s][j] = l;
+        for (int j = 0; j < 2; j++) {
+            const float y[4] = {x[s][j].x, x[s][j].y, x[s][j].z, x[s][j].w};
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                _Float16 h, l;
+                ck_split(y[d] * up, h, l);
+                hi[s][4 * j + d] = h;
+                lo[s][4 * j + d] = l;
+            }
         }
     return down * scale;
 }

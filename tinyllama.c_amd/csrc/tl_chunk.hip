@@ -67,6 +67,12 @@ int tl_chunk_check(const LayerView &L, const tl_chunk *ch, u32 n_chunk, u32 rows
     return TL_OK;
 }
 
+/* the starts of the launch's chunks side by side */
+template <class P>
+static void starts(P &p) {
+    for (u32 i = 0; i < CK_MAX_SEQ; i++) p.wg0[i] = i < p.n_seq ? p.seq[i].wg0 : ~0u;
+}
+
 static CkCache cache_of(const LayerView &L, u32 shift) {
     CkCache c;
     c.k = (const u16 *)L.k;
@@ -108,6 +114,7 @@ static int check_rows(const char *what, const void *p, u32 stride, u64 width) {
 /* ------------------------------------------------------------------------ */
 
 struct CkAppendParams {
+    u32 wg0[CK_MAX_SEQ];
     CkSeq seq[CK_MAX_SEQ];
     CkCache c;
     const float *q, *k, *v, *qw, *kw;
@@ -128,7 +135,7 @@ template <int D, bool Q8>
 __global__ __launch_bounds__(256) void chunk_append_kernel(const CkAppendParams p) {
     constexpr u32 LPR = D / 8, GRP = 256 / LPR;
     __shared__ float2 s_cs[D / 2];
-    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 r = blockIdx.x - sq.wg0;
     const u32 key = sq.pos + r;
     const u64 brow = (u64)sq.row + r;
@@ -286,6 +293,7 @@ static int norm_append(const LayerView &L, const tl_qk_norm_args *a, const tl_ch
         }
         if (!m) break;
         p.n_seq = m;
+        starts(p);
         /* few rows: their heads over several workgroups */
         const u32 units = a->n_head + 2 * L.n_kv_head, per = 256 / (L.head_dim / 8);
         u32 split = (units + per - 1) / per;
@@ -335,9 +343,9 @@ struct AttnPlan {
 /* More columns than this take the wide kernel. */
 #define CK_WIDE_MIN 32
 
-/* As many splits as fill the chip with two workgroups to a CU (one at
- * head_dim 256), none of fewer keys than 128 (one tile for each narrow wave) or
- * 256 (wide: partial rows of 128 columns cost more to join). */
+/* As many splits as fill the chip (narrow: one workgroup to a CU, wide: two, at
+ * head_dim 256 one), none of fewer tiles than a narrow workgroup has waves, or
+ * of fewer keys than 256 (wide: partial rows of 128 columns cost more to join). */
 static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
                       u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
@@ -353,11 +361,23 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
         tiles[w][pl.n[w]++] = span_tiles(*ch[i], window, 0, ch[i]->n);
         total[w] += tiles[w][pl.n[w] - 1] * s.ncb * n_kv;
     }
-    const u32 fill = head_dim == 256 ? 256 : 512;
     for (int w = 0; w < 2; w++) {
+        const u32 fill = w && head_dim != 256 ? 512 : 256;
         u64 per = (total[w] + fill - 1) / fill, wgs = 0;
-        const u64 least = w ? 8 : 4;
+        const u64 least = w || head_dim != 256 ? 8 : 4;
         if (per < least) per = least;
+        /* the smallest share whose workgroups all run at once, if there is one */
+        u64 all = 0, most = 0;
+        for (u32 i = 0; i < pl.n[w]; i++) {
+            all += (u64)pl.seq[w][i].ncb * n_kv;
+            most = tiles[w][i] > most ? tiles[w][i] : most;
+        }
+        for (; all <= fill && per < most; per += 1 + per / 32) {
+            u64 at_once = 0;
+            for (u32 i = 0; i < pl.n[w]; i++)
+                at_once += (u64)pl.seq[w][i].ncb * n_kv * ((tiles[w][i] + per - 1) / per);
+            if (at_once <= fill) break;
+        }
         for (u32 i = 0; i < pl.n[w]; i++) {
             CkSeq &s = pl.seq[w][i];
             u64 ns = (tiles[w][i] + per - 1) / per;
@@ -505,6 +525,7 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
             if (!pl.wgs[w]) continue;
             p.n_seq = pl.n[w];
             memcpy(p.seq, pl.seq[w], pl.n[w] * sizeof(CkSeq));
+            starts(p);
             if (w) ck_launch_wide(p, L.head_dim, L.q8, pl.wgs[w], st);
             else ck_launch_attn(p, L.head_dim, L.q8, pl.wgs[w], st);
             HIP_TRY(hipGetLastError());
@@ -521,6 +542,7 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
                 }
             if (!k) continue;
             p.n_seq = k;
+            starts(p);
             ck_launch_merge(p, L.head_dim, (u32)blocks, st);
             HIP_TRY(hipGetLastError());
         }
@@ -571,6 +593,7 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
             wgs += ((u64)p.seq[j].pos + p.seq[j].n + CK_KEYS - 1) / CK_KEYS;
         }
         if (wgs > 0x7fffffffull) return tl_fail(TL_ERANGE, "attn_weight: too many keys");
+        starts(p);
         ck_launch_weight(p, L.head_dim, L.q8, (u32)wgs, st);
         HIP_TRY(hipGetLastError());
     }

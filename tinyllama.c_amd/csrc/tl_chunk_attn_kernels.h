@@ -6,7 +6,8 @@
 #pragma once
 #include "tl_chunk.h"
 
-#define CK_WAVES 4
+/* waves of a narrow workgroup: one workgroup to a CU */
+#define CK_WAVES(D) ((D) == 256 ? 4 : 8)
 
 /* the maximum moves only when a score passes it by more than 2^CK_LAZY, and
  * probabilities are taken against 2^CK_UP below it: they reach 2^15 at most, so
@@ -15,15 +16,15 @@
 #define CK_UP 7.f
 
 template <int D, bool Q8, bool BIAS>
-__global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_kernel(const CkAttnParams p) {
-    constexpr int KS = D / 32, NM = D / 16;
+__global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const CkAttnParams p) {
+    constexpr int KS = D / 32, NM = D / 16, NW = CK_WAVES(D), NT = 64 * NW;
     constexpr int ROWF = D + 4;
-    __shared__ float s_o[CK_WAVES][CK_COLS][ROWF];
-    __shared__ float s_m[CK_WAVES][CK_COLS], s_l[CK_WAVES][CK_COLS];
+    __shared__ __align__(16) float s_o[NW * CK_COLS * ROWF];
+    __shared__ float s_m[NW][CK_COLS], s_l[NW][CK_COLS];
     __shared__ u32 s_last;
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u32 i = lane & 15, g = lane >> 4;
-    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
@@ -35,12 +36,6 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     const u32 pq = sq.pos + r, end = sq.pos + sq.n;
     const u64 brow = (u64)sq.row + r;
 
-    h8_t qh[KS], ql[KS];
-    float cs = ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
-    if constexpr (!BIAS) cs *= CK_LOG2E;
-    const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
-    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
-
     CkSees see;
     see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
     CkSpan span;
@@ -49,11 +44,6 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     tiles.set(span);
     const u32 n_tiles = tiles.count();
     const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
-
-    float m = -INFINITY, l = 0.f;
-    f4_t o[NM];
-#pragma unroll
-    for (int j = 0; j < NM; j++) o[j] = (f4_t){0.f, 0.f, 0.f, 0.f};
 
     CkTile<D, Q8> tile;
     /* lane's key of a tile (the upper half of the wave repeats the lower) */
@@ -69,22 +59,34 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
 #pragma unroll
         for (int e = 0; e < 8; e++) rv[e] = __shfl(row, 8 * g + e);
     };
+    /* the first tile's rows, q, then the tile itself are requested before q is used */
     u32 t = t0 + wave;
     u32 row = 0, next = 0;
+    if (t < t1) row = look(t);
+    float4 qx[KS][2];
+    ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, qx);
+    const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
     if (t < t1) {
-        row = look(t);
         const u32 rc = row < p.c.cap ? row : 0;
         u32 rk[2], rv[8];
         rows_k(rc, rk);
         tile.load_k(p.c, kvh, rk, g);
         rows_v(rc, rv);
         tile.load_v(p.c, kvh, rv, i);
-        if (t + CK_WAVES < t1) next = look(t + CK_WAVES);
+        if (t + NW < t1) next = look(t + NW);
     }
-    for (; t < t1; t += CK_WAVES) {
+    h8_t qh[KS], ql[KS];
+    float cs = ck_split_q<D, 4>(qx, p.scale, qh, ql);
+    if constexpr (!BIAS) cs *= CK_LOG2E;
+    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+    float m = -INFINITY, l = 0.f;
+    f4_t o[NM];
+#pragma unroll
+    for (int j = 0; j < NM; j++) o[j] = (f4_t){0.f, 0.f, 0.f, 0.f};
+    for (; t < t1; t += NW) {
         const u32 kb = tiles.key(t);
         const u64 bad = __ballot(row >= p.c.cap);
-        const bool more = t + CK_WAVES < t1;
+        const bool more = t + NW < t1;
         float x[8];
 #pragma unroll
         for (int a = 0; a < 2; a++) {
@@ -166,7 +168,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             rows_v(rn, rv);
             tile.load_v(p.c, kvh, rv, i);
             row = next;
-            if (t + 2 * CK_WAVES < t1) next = look(t + 2 * CK_WAVES);
+            if (t + 2 * NW < t1) next = look(t + 2 * NW);
         }
     }
     l += __shfl_xor(l, 16);
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     for (int e = 0; e < 4; e++)
 #pragma unroll
         for (int j = 0; j < NM; j += 4)
-            *(float4 *)&s_o[wave][i][NM * (4 * g + e) + j] =
+            *(float4 *)&s_o[(wave * CK_COLS + i) * ROWF + NM * (4 * g + e) + j] =
                 make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
     __syncthreads();
     constexpr u32 V4 = D / 4;
@@ -190,18 +192,28 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
     const u64 part = (u64)sq.part0 + (u64)group * sq.ns * CK_COLS;      /* the group's first partial row */
     const __amdgpu_buffer_rsrc_t ra = buf_rsrc(p.ws_acc + part * D);
     const __amdgpu_buffer_rsrc_t rm = buf_rsrc(p.ws_ml + part);
-    for (u32 u = threadIdx.x; u < units; u += 64 * CK_WAVES) {
+    auto write = [&](u32 c, u32 d, float4 a, float sum, float M) {
+        const u32 cc = c0 + c, rr = cc / p.gqa, hh = kvh * p.gqa + cc % p.gqa;
+        const u64 br = (u64)sq.row + rr;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
+            make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        if (p.lse && d == 0)
+            p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY
+                : ((M == -INFINITY ? 0.f : M) - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
+    };
+    for (u32 u = threadIdx.x; u < units; u += NT) {
         const u32 c = u / V4, d = u % V4;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < CK_WAVES; w++) M = fmaxf(M, s_m[w][c]);
+        for (int w = 0; w < NW; w++) M = fmaxf(M, s_m[w][c]);
         const float M0 = M == -INFINITY ? 0.f : M;
         float sum = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < CK_WAVES; w++) {
+        for (int w = 0; w < NW; w++) {
             const float f = __builtin_amdgcn_exp2f(s_m[w][c] - M0);
-            const float4 v = *(const float4 *)&s_o[w][c][4 * d];
+            const float4 v = *(const float4 *)&s_o[(w * CK_COLS + c) * ROWF + 4 * d];
             sum = fmaf(f, s_l[w][c], sum);
             a.x = fmaf(f, v.x, a.x);
             a.y = fmaf(f, v.y, a.y);
@@ -209,13 +221,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             a.w = fmaf(f, v.w, a.w);
         }
         if (sq.ns == 1) {
-            const u32 cc = c0 + c, rr = cc / p.gqa, hh = kvh * p.gqa + cc % p.gqa;
-            const u64 br = (u64)sq.row + rr;
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
-                make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            if (p.lse && d == 0)
-                p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
+            write(c, d, a, sum, M);
         } else {
             const u32x4v_t v = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(a.z), __float_as_uint(a.w)};
             __builtin_amdgcn_raw_buffer_store_b128(v, ra, ((split * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
@@ -226,7 +232,9 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
         }
     }
     if (sq.ns == 1) return;
-    /* the last split of the group to arrive joins them all */
+    /* the last split of the group to arrive joins them all: `parts` threads to
+     * a float4 of the output, each with a run of the splits, eight of them
+     * requested at a time; then the parts through LDS, in order */
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     u32 *cnt = p.cnt + (u64)(sq.grp0 + group) * CK_CNT_PAD;
@@ -234,11 +242,17 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
         s_last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sq.ns - 1;
     __syncthreads();
     if (!s_last) return;
-    for (u32 u = threadIdx.x; u < units; u += 64 * CK_WAVES) {
+    u32 parts = 1;
+    while (parts < NW && parts * 2 * units <= NT && parts * 8 < sq.ns) parts *= 2;
+    const u32 run = (sq.ns + parts - 1) / parts;
+    const u32 lanes = parts == 1 ? NT : NT / parts;
+    const u32 pi = threadIdx.x / lanes;
+    for (u32 u = threadIdx.x % lanes; u < units; u += lanes) {
         const u32 c = u / V4, d = u % V4;
         float M = -INFINITY, sum = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (u32 s0 = 0; s0 < sq.ns; s0 += 8) {
+        const u32 s1 = min((pi + 1) * run, sq.ns);
+        for (u32 s0 = pi * run; s0 < s1; s0 += 8) {
             u32x2v_t ml[8];
             u32x4v_t v[8];
 #pragma unroll
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const u32 mb = ml[j][0];
-                Mn = fmaxf(Mn, s0 + j < sq.ns ? __uint_as_float(mb) : -INFINITY);
+                Mn = fmaxf(Mn, s0 + j < s1 ? __uint_as_float(mb) : -INFINITY);
             }
             const float M0 = Mn == -INFINITY ? 0.f : Mn;
             const float f0 = __builtin_amdgcn_exp2f(M - M0);
@@ -259,7 +273,7 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                if (s0 + j >= sq.ns) break;
+                if (s0 + j >= s1) break;
                 const u32 mb = ml[j][0], lb = ml[j][1];
                 const u32 v0 = v[j][0], v1 = v[j][1], v2 = v[j][2], v3 = v[j][3];
                 const float f = __builtin_amdgcn_exp2f(__uint_as_float(mb) - M0);
@@ -271,14 +285,35 @@ __global__ __launch_bounds__(64 * CK_WAVES, D == 256 ? 1 : 2) void chunk_attn_ke
             }
             M = Mn;
         }
-        const u32 cc = c0 + c, rr = cc / p.gqa, hh = kvh * p.gqa + cc % p.gqa;
-        const u64 br = (u64)sq.row + rr;
-        const float M0 = M == -INFINITY ? 0.f : M;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
-            make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-        if (p.lse && d == 0)
-            p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY : (M0 - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
+        if (parts == 1) {
+            write(c, d, a, sum, M);
+        } else {
+            *(float4 *)&s_o[(pi * CK_COLS + c) * ROWF + 4 * d] = a;
+            if (d == 0) {
+                s_m[pi][c] = M;
+                s_l[pi][c] = sum;
+            }
+        }
+    }
+    if (parts > 1) {
+        __syncthreads();
+        for (u32 u = threadIdx.x; u < units; u += NT) {
+            const u32 c = u / V4, d = u % V4;
+            float M = -INFINITY, sum = 0.f;
+            for (u32 w = 0; w < parts; w++) M = fmaxf(M, s_m[w][c]);
+            const float M0 = M == -INFINITY ? 0.f : M;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (u32 w = 0; w < parts; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_m[w][c] - M0);
+                const float4 v = *(const float4 *)&s_o[(w * CK_COLS + c) * ROWF + 4 * d];
+                sum = fmaf(f, s_l[w][c], sum);
+                a.x = fmaf(f, v.x, a.x);
+                a.y = fmaf(f, v.y, a.y);
+                a.z = fmaf(f, v.z, a.z);
+                a.w = fmaf(f, v.w, a.w);
+            }
+            write(c, d, a, sum, M);
+        }
     }
     if (threadIdx.x == 0)
         __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -340,7 +375,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     __shared__ u64 s_odd[2][2];      /* keys of a tile whose V is not all finite */
     const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
     const u32 i = lane & 31, h = lane >> 5;
-    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
@@ -352,7 +387,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     const u64 brow = (u64)sq.row + r;
 
     h8_t qh[NS], ql[NS];
-    float cs = ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, p.scale, qh, ql);
+    float4 qx[NS][2];
+    ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
+    float cs = ck_split_q<D, 2>(qx, p.scale, qh, ql);
     if constexpr (!BIAS) cs *= CK_LOG2E;
     const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
     const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
@@ -655,7 +692,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
 template <int D>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(const CkAttnParams p) {
     constexpr u32 V4 = D / 4, CPB = 256 / V4;
-    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 at = (blockIdx.x - sq.wg0) * CPB + threadIdx.x / V4, d = threadIdx.x % V4;
     const u32 cols = sq.n * p.gqa;
     const u32 kvh = at / cols, col = at % cols;

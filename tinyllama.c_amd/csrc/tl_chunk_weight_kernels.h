@@ -14,7 +14,7 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
     __shared__ float s_sum[4][CK_KEYS];
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u32 i = lane & 15, g = lane >> 4;
-    const CkSeq &sq = p.seq[ck_find(p.seq, p.n_seq, blockIdx.x)];
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 kb = (blockIdx.x - sq.wg0) * CK_KEYS;
     const u32 end = sq.pos + sq.n, cols = sq.n * p.gqa;
     const u32 key = kb + (lane & 31);
@@ -43,7 +43,9 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
             for (int e = 0; e < 8; e++) any |= see.sees(kb + 8 * g + e);
             if (!__any(any && real)) continue;
             h8_t qh[KS], ql[KS];
-            float cs = ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, p.scale, qh, ql);
+            float4 qx[KS][2];
+            ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, qx);
+            float cs = ck_split_q<D, 4>(qx, p.scale, qh, ql);
             if constexpr (!BIAS) cs *= CK_LOG2E;
             const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
             const float lse = p.lse[brow * p.n_head + head] * CK_LOG2E;
