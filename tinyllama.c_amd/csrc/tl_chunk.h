@@ -94,10 +94,13 @@ TL_DEV float ck_tanh(float x) {
     return ax < 0.25f ? small : big;
 }
 
-/* f32 as a pair of f16 whose sum has 22 bits of it */
-TL_DEV void ck_split(float x, _Float16 &hi, _Float16 &lo) {
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
+/* two f32 as pairs of f16 whose sums have 22 bits of them (x - hi is exact, one
+ * mixed-precision fma) */
+TL_DEV void ck_split2(float x, float y, u32 &hi, u32 &lo) {
+    const tl_f16x2_t h = __builtin_convertvector((tl_f32x2_t){x, y}, tl_f16x2_t);
+    const tl_f32x2_t r = {fmaf((float)h.x, -1.f, x), fmaf((float)h.y, -1.f, y)};
+    hi = __builtin_bit_cast(u32, h);
+    lo = __builtin_bit_cast(u32, __builtin_convertvector(r, tl_f16x2_t));
 }
 
 /* power of two that brings a row's largest |x| to [2^14, 2^15), so that both
@@ -382,18 +385,21 @@ TL_DEV float ck_split_q(const float4 (&x)[D / (8 * G)][2], float scale, h8_t (&h
     const float up = __uint_as_float((u32)(e + 127) << 23);
     const float down = __uint_as_float((u32)(127 - e) << 23);
 #pragma unroll
-    for (int s = 0; s < N; s++)
+    for (int s = 0; s < N; s++) {
+        u4_t hw, lw;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const float y[4] = {x[s][j].x, x[s][j].y, x[s][j].z, x[s][j].w};
-#pragma unroll
-            for (int d = 0; d < 4; d++) {
-                _Float16 h, l;
-                ck_split(y[d] * up, h, l);
-                hi[s][4 * j + d] = h;
-                lo[s][4 * j + d] = l;
-            }
+            u32 h[2], l[2];
+            ck_split2(x[s][j].x * up, x[s][j].y * up, h[0], l[0]);
+            ck_split2(x[s][j].z * up, x[s][j].w * up, h[1], l[1]);
+            hw[2 * j] = h[0];
+            hw[2 * j + 1] = h[1];
+            lw[2 * j] = l[0];
+            lw[2 * j + 1] = l[1];
         }
+        hi[s] = __builtin_bit_cast(h8_t, hw);
+        lo[s] = __builtin_bit_cast(h8_t, lw);
+    }
     return down * scale;
 }
 

@@ -145,16 +145,20 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
             m = mn;
         }
         const float mref = m == -INFINITY ? 0.f : m - CK_UP;
-        h8_t ph, pl;
+        u4_t pw, qw;
+        float l1 = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float pe = __builtin_amdgcn_exp2f(x[e] - mref);
-            l += pe;
-            _Float16 a, b;
-            ck_split(pe, a, b);
-            ph[e] = a;
-            pl[e] = b;
+        for (int e = 0; e < 8; e += 2) {
+            const float a = __builtin_amdgcn_exp2f(x[e] - mref), b = __builtin_amdgcn_exp2f(x[e + 1] - mref);
+            l += a;
+            l1 += b;
+            u32 hi, lo;
+            ck_split2(a, b, hi, lo);
+            pw[e >> 1] = hi;
+            qw[e >> 1] = lo;
         }
+        l += l1;
+        const h8_t ph = __builtin_bit_cast(h8_t, pw), pl = __builtin_bit_cast(h8_t, qw);
 #pragma unroll
         for (int j = 0; j < NM; j++) {
             h8_t vh, vl;
@@ -326,12 +330,16 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
  * >> 5).  A lane's sixteen scores of a 32-key block are rows (r & 3) + 8 (r >>
  * 2) + 4 h; matrix row rho is fed key rho with bits 2 and 3 exchanged, so they
  * are keys 16 u + 8 h + j (r = 8 u + j), the k order of step u of the second
- * product.  Waves 0 and 1 fetch a tile's K rows, waves 2 and 3 its V rows, eight
- * keys to a lane, which they transpose on the way to LDS (v_perm on pairs), so
- * that both operands are 16-byte reads.  Units of 16 bytes are permuted within a
- * row so that 16 lanes' reads cover all banks.  Two buffers, one barrier per
- * tile; a tile's rows are looked up two tiles ahead, its data fetched one ahead.
- * A Q8_0 tile is kept as two planes, hi and lo. */
+ * product.
+ *
+ * Tiles of KT keys, two buffers, one barrier each.  The pool rows of a tile are
+ * looked up by one wave three tiles ahead and handed on through LDS; K rows go
+ * straight to LDS (LDS-direct loads, one tile ahead); V goes through registers,
+ * eight keys to a lane, which transposes them on the way to LDS (v_perm on
+ * pairs), so that both operands are 16-byte reads, four requested ahead of the
+ * matrix instructions.  16-byte units are permuted within a row so that 16
+ * lanes' reads cover all banks.  A Q8_0 tile is kept as two planes, hi and lo,
+ * both through registers (waves 0 and 1 K, waves 2 and 3 V). */
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
 template <int D, bool Q8>
@@ -340,19 +348,19 @@ struct CkWide {
     static constexpr int U = D / 8;                  /* 16-byte units of a K row in LDS */
     static constexpr int VU = KT / 8;                /* ... of a V^T row */
     static constexpr int PL = Q8 ? 2 : 1;
-    static constexpr int DPL = KT * D / 1024;        /* dims of V of a staging lane */
+    static constexpr int VL = Q8 ? 128 : 256;        /* lanes that stage V */
+    static constexpr int DPL = KT * D / 8 / VL;      /* dims of V of one of them */
     static constexpr int RU = Q8 ? D / 16 : D / 8;   /* 16-byte units of a K row in memory */
-    static constexpr int KL = KT * RU / 128;         /* ... of a staging lane */
-    static constexpr int VD = Q8 ? DPL / 4 : DPL / 2;   /* dwords of V of a key and staging lane */
-    static constexpr int ST = KL * 4 > 8 * VD ? KL * 4 : 8 * VD;
+    static constexpr int KL = Q8 ? KT * RU / 128 : KT * D / 2048;   /* ... of a lane (Q8_0), of a wave / 64 */
+    static constexpr int VD = Q8 ? DPL / 4 : DPL / 2;   /* dwords of V of a key and lane */
+    static constexpr int ST = Q8 && KL * 4 > 8 * VD ? KL * 4 : 8 * VD;
     static constexpr int SC = Q8 ? 8 : 1;            /* scales of a staging lane */
-    static_assert(DPL == 4 || DPL == 8, "staging");
+    static_assert(Q8 ? DPL == 4 || DPL == 8 : DPL == 2 || DPL == 4, "staging");
     static constexpr int KP = KT * U * 16, VP = D * VU * 16;   /* bytes of a plane */
     /* byte offsets of units; exclusive-or linear in the bits of their arguments, so
      * an offset is the lane's part with a constant part put in (put) */
-    static constexpr TL_HOSTDEV u32 kat(u32 key, u32 unit) {
-        return (key * U + (unit ^ (U == 8 ? (key >> 1) & 7 : key & 15))) * 16;
-    }
+    static constexpr TL_HOSTDEV u32 kswz(u32 key) { return U == 8 ? (key >> 1) & 7 : key & 15; }
+    static constexpr TL_HOSTDEV u32 kat(u32 key, u32 unit) { return (key * U + (unit ^ kswz(key))) * 16; }
     static constexpr TL_HOSTDEV u32 vat(u32 dim, u32 unit) {
         return (dim * VU + (unit ^ (VU == 8 ? ((dim >> 1) ^ (dim >> 3)) & 7 : (dim >> 2) & 3))) * 16;
     }
@@ -364,6 +372,17 @@ struct CkWide {
     }
 };
 
+/* 64 lanes' 16 bytes at base + off straight to LDS at `to` (wave-uniform) + 16
+ * lane; the caller waits (vmcnt) before the barrier that hands them on */
+TL_DEV void ck_lds_load16(void *to, const void *base, u32 off) {
+    const u64 g = (u64)base;
+    const void *sb = (const void *)(((u64)ck_uniform((u32)(g >> 32)) << 32) | ck_uniform((u32)g));
+    const u32 m0 = ck_uniform((u32)(u64)(__attribute__((address_space(3))) char *)to);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "{m0}"(m0) : "memory");
+}
+
+#define CK_AHEAD 4   /* LDS operand reads in flight ahead of the matrix instructions */
+
 template <int D, bool Q8, bool BIAS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
     typedef CkWide<D, Q8> W;
@@ -371,8 +390,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     /* buffer b, plane l of K: s_k + (b * PL + l) * KP; of V the same */
     __shared__ __align__(16) char s_k[2 * W::PL * W::KP];
     __shared__ __align__(16) char s_v[2 * W::PL * W::VP];
+    __shared__ __align__(16) u32 s_row[2][KT];   /* pool rows of a tile's keys, 0 for the bad ones */
+    __shared__ u64 s_bad[4];                     /* keys of a tile without a row */
+    __shared__ u64 s_odd[2][4];                  /* keys of a tile whose V is not all finite */
     __shared__ CkSpan s_span[4];
-    __shared__ u64 s_odd[2][2];      /* keys of a tile whose V is not all finite */
     const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
     const u32 i = lane & 31, h = lane >> 5;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
@@ -382,20 +403,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     const u32 cols = sq.n * p.gqa, cw = cb * CK_WCOLS + wave * 32;
     const bool live = cw < cols;
     const u32 col = min(cw + i, cols - 1);
-    const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
-    const u32 pq = sq.pos + r, end = sq.pos + sq.n;
-    const u64 brow = (u64)sq.row + r;
-
+    const u32 end = sq.pos + sq.n;
+    u32 pq;
     h8_t qh[NS], ql[NS];
-    float4 qx[NS][2];
-    ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
-    float cs = ck_split_q<D, 2>(qx, p.scale, qh, ql);
-    if constexpr (!BIAS) cs *= CK_LOG2E;
-    const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
+    float cs, slope = 0.f;
+    CkSees see;
+    {
+        const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+        const u64 brow = (u64)sq.row + r;
+        pq = sq.pos + r;
+        see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
+        if (BIAS && p.slopes) slope = p.slopes[head];
+        float4 qx[NS][2];
+        ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
+        cs = ck_split_q<D, 2>(qx, p.scale, qh, ql);
+        if constexpr (!BIAS) cs *= CK_LOG2E;
+    }
     const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
 
-    CkSees see;
-    see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
     CkSpan span, all;
     span.set<32>(see);
     if (lane == 0) s_span[wave] = span;
@@ -411,12 +436,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
         all.min_hi = min(all.min_hi, o.min_hi);
         all.max_f = max(all.max_f, o.max_f);
     }
+    all.fmin = ck_uniform(all.fmin);
+    all.lo = ck_uniform(all.lo);
+    all.hi = ck_uniform(all.hi);
+    all.max_lo = ck_uniform(all.max_lo);
+    all.min_hi = ck_uniform(all.min_hi);
+    all.max_f = ck_uniform(all.max_f);
+    all.pre = ck_uniform(all.pre);
     CkTiles<KT> tiles;
     tiles.set(all);
-    tiles.a0 = ck_uniform(tiles.a0);
-    tiles.na = ck_uniform(tiles.na);
-    tiles.b0 = ck_uniform(tiles.b0);
-    tiles.nb = ck_uniform(tiles.nb);
     const u32 n_tiles = tiles.count();
     const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
 
@@ -430,58 +458,76 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     /* staging */
     u32 st[W::ST];
     u32 sc[W::SC];
-    const u32 sl = (wave & 1) * 64 + lane;
-    const u32 dg = sl % (D / W::DPL), kg = sl / (D / W::DPL);      /* V: dims and keys of the lane */
     const char *kbase = (const char *)p.c.k + (u64)kvh * p.c.cap * (Q8 ? D : 2 * D);
     const char *vbase = (const char *)p.c.v + (u64)kvh * p.c.cap * (Q8 ? D : 2 * D);
     const u16 *ksb = p.c.ks + (u64)kvh * p.c.cap * (D / 32);
     const u16 *vsb = p.c.vs + (u64)kvh * p.c.cap * (D / 32);
-    const u32 kst = W::kat(sl / W::RU, (Q8 ? 2 : 1) * (sl % W::RU)), vst = W::vat(dg * W::DPL, kg);
+    /* lane's pool row of a tile (KT = 32: the upper half repeats the lower) */
     auto look = [&](u32 t) -> u32 {
         const u32 key = tiles.key(t) + (lane & (KT - 1));
         return key < end ? ck_row(p.c, sq.pages, key) : ~0u;
     };
-    auto fetch = [&](u32 rc) {
-        if (wave < 2) {
+    auto hand_on = [&](u32 t, u32 row) {     /* by one wave */
+        const u64 bad = __ballot(row >= p.c.cap);
+        if (lane < KT) s_row[(t - t0) & 1][lane] = row < p.c.cap ? row : 0;
+        if (lane == 0) s_bad[(t - t0) & 3] = bad;
+    };
+    /* the places of a staging lane, kept out of registers across the tile loop */
+    auto place = [&](u32 &sl) {
+        sl = Q8 ? (wave & 1) * 64 + lane : threadIdx.x;
+        asm volatile("" : "+v"(sl));
+    };
+    auto fetch = [&](u32 t) {
+        const u32 *rows = s_row[(t - t0) & 1];
+        u32 sl;
+        place(sl);
+        const u32 dg = sl % (D / W::DPL), kg = sl / (D / W::DPL);      /* V: dims and keys of the lane */
+        if constexpr (!Q8) {
+            char *to = s_k + ((t - t0) & 1) * W::KP;
+            const u32 ln = sl & 63;
 #pragma unroll
             for (int j = 0; j < W::KL; j++) {
-                const u32 x = j * 128 + sl, key = x / W::RU, u = x % W::RU;
-                const u32 row = __shfl(rc, key);
+                const u32 c = wave * W::KL + j, key = c * (64 / W::U) + ln / W::U;
+                ck_lds_load16(to + c * 1024, kbase, rows[key] * (u32)(2 * D) + ((ln % W::U) ^ W::kswz(key)) * 16);
+            }
+        } else if (wave < 2) {
+#pragma unroll
+            for (int j = 0; j < W::KL; j++) {
+                const u32 u = sl % W::RU, row = rows[j * (128 / W::RU) + sl / W::RU];
                 const u4_t v = *(const u4_t *)(kbase + (u64)(row * (u32)(W::RU * 16) + u * 16));
 #pragma unroll
                 for (int d = 0; d < 4; d++) st[4 * j + d] = v[d];
-                if constexpr (Q8) sc[j] = ksb[(u64)(row * (u32)(D / 32) + (u >> 1))];
+                sc[j] = ksb[(u64)(row * (u32)(D / 32) + (u >> 1))];
             }
-        } else {
+            return;
+        }
+        const u4_t ra = *(const u4_t *)(rows + 8 * kg), rb = *(const u4_t *)(rows + 8 * kg + 4);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const u32 row = __shfl(rc, 8 * kg + e);
-                const char *a = vbase + (u64)(row * (u32)(Q8 ? D : 2 * D) + dg * (Q8 ? W::DPL : 2 * W::DPL));
-                if constexpr (W::VD == 1) {
-                    st[e] = *(const u32 *)a;
-                } else if constexpr (W::VD == 2) {
-                    const uint2 v = *(const uint2 *)a;
-                    st[2 * e] = v.x;
-                    st[2 * e + 1] = v.y;
-                } else {
-                    const u4_t v = *(const u4_t *)a;
-#pragma unroll
-                    for (int d = 0; d < 4; d++) st[4 * e + d] = v[d];
-                }
-                if constexpr (Q8) sc[e] = vsb[(u64)(row * (u32)(D / 32) + dg * W::DPL / 32)];
+        for (int e = 0; e < 8; e++) {
+            const u32 row = e < 4 ? ra[e & 3] : rb[e & 3];
+            const char *a = vbase + (u64)(row * (u32)(Q8 ? D : 2 * D) + dg * (Q8 ? W::DPL : 2 * W::DPL));
+            if constexpr (W::VD == 1) {
+                st[e] = *(const u32 *)a;
+            } else {
+                const uint2 v = *(const uint2 *)a;
+                st[2 * e] = v.x;
+                st[2 * e + 1] = v.y;
             }
+            if constexpr (Q8) sc[e] = vsb[(u64)(row * (u32)(D / 32) + dg * W::DPL / 32)];
         }
     };
-    /* bad: keys of the tile without a row; check: V may be seen by some columns only */
-    auto store = [&](u32 buf, u64 bad, bool check) {
-        if (wave < 2) {
-#pragma unroll
-            for (int j = 0; j < W::KL; j++) {
+    auto store = [&](u32 t) {
+        const u32 buf = (t - t0) & 1;
+        u32 sl;
+        place(sl);
+        const u32 dg = sl % (D / W::DPL), kg = sl / (D / W::DPL);
+        if constexpr (Q8)
+            if (wave < 2) {
+                const u32 kst = W::kat(sl / W::RU, 2 * (sl % W::RU));
                 char *to = s_k + buf * (W::PL * W::KP);
-                const u32 c = W::kat(j * (128 / W::RU), 0);
-                if constexpr (!Q8) {
-                    *(u4_t *)(to + W::kput(kst, c)) = (u4_t){st[4 * j], st[4 * j + 1], st[4 * j + 2], st[4 * j + 3]};
-                } else {
+#pragma unroll
+                for (int j = 0; j < W::KL; j++) {
+                    const u32 c = W::kat(j * (128 / W::RU), 0);
                     const tl_half2 d2 = __builtin_bit_cast(tl_half2, sc[j] * 0x10001u);
                     u32 hi[8], lo[8];
 #pragma unroll
@@ -495,39 +541,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                     for (int z = 0; z < 2; z++) {
                         char *at = to + W::kput(kst, c ^ (z * 16));
                         *(u4_t *)at = (u4_t){hi[4 * z], hi[4 * z + 1], hi[4 * z + 2], hi[4 * z + 3]};
-                        *(u4_t *)(at + (W::PL - 1) * W::KP) = (u4_t){lo[4 * z], lo[4 * z + 1], lo[4 * z + 2], lo[4 * z + 3]};
+                        *(u4_t *)(at + W::KP) = (u4_t){lo[4 * z], lo[4 * z + 1], lo[4 * z + 2], lo[4 * z + 3]};
                     }
                 }
+                return;
             }
-            return;
-        }
-        if (bad) {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if ((bad >> (8 * kg + e)) & 1) {
-#pragma unroll
-                    for (int d = 0; d < W::VD; d++) st[W::VD * e + d] = 0;
-                    if constexpr (Q8) sc[e] = 0;
-                }
-        }
-        if (check) {
-            /* infinities and NaN, which only some columns may see: zeros in the
-             * product, and the columns that do see the key are told */
+        const u64 bad = s_bad[(t - t0) & 3];
+        if (bad || !all.full(tiles.key(t), KT)) {
+            /* keys without a row are zeros; infinities and NaN, which only some
+             * columns may see, are zeros in the product, and the columns that do
+             * see the key are told */
             u32 odd = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
+                const bool none = (bad >> (8 * kg + e)) & 1;
                 bool x = false;
                 if constexpr (Q8) {
                     x = (sc[e] & 0x7fffu) > 0x6006u;
-                    sc[e] = x ? 0 : sc[e];
+                    sc[e] = x || none ? 0 : sc[e];
                 } else {
 #pragma unroll
                     for (int d = 0; d < W::VD; d++)
                         x |= (st[W::VD * e + d] & 0x7c00u) == 0x7c00u || (st[W::VD * e + d] & 0x7c000000u) == 0x7c000000u;
-#pragma unroll
-                    for (int d = 0; d < W::VD; d++) st[W::VD * e + d] = x ? 0 : st[W::VD * e + d];
                 }
-                odd |= (u32)x << e;
+#pragma unroll
+                for (int d = 0; d < W::VD; d++) st[W::VD * e + d] = x || none ? 0 : st[W::VD * e + d];
+                odd |= (u32)(x && !none) << e;
             }
             u64 keys = 0;
             if (__any(odd)) {
@@ -535,8 +574,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
 #pragma unroll
                 for (int x = 1; x < 64; x <<= 1) keys |= __shfl_xor(keys, x);
             }
-            if (lane == 0) s_odd[buf][wave - 2] = keys;
+            if (lane == 0) s_odd[buf][wave] = keys;
         }
+        const u32 vst = W::vat(dg * W::DPL, kg);
 #pragma unroll
         for (int x = 0; x < W::DPL; x++) {
             u4_t hi, lo;
@@ -558,62 +598,76 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
             }
             char *at = s_v + buf * (W::PL * W::VP) + W::vput(vst, W::vat(x, 0));
             *(u4_t *)at = hi;
-            if constexpr (Q8) *(u4_t *)(at + (W::PL - 1) * W::VP) = lo;
+            if constexpr (Q8) *(u4_t *)(at + W::VP) = lo;
         }
     };
 
-    const u32 krd = W::kat((i & 19) | ((i & 4) << 1) | ((i & 8) >> 1), h), vrd = W::vat(i, h);
     u32 next = 0;
-    u64 bad = 0;
     if (t0 < t1) {
-        const u32 row = look(t0);
-        bad = __ballot(row >= p.c.cap);
-        fetch(row < p.c.cap ? row : 0);
-        if (t0 + 1 < t1) next = look(t0 + 1);
-        store(0, bad, bad || !all.full(tiles.key(t0), KT));
-    }
-    for (u32 t = t0; t < t1; t++) {
-        const u32 buf = (t - t0) & 1;
-        const u32 kt = tiles.key(t);
-        const bool more = t + 1 < t1;
+        if (wave == 0) {
+            const u32 a = look(t0), b = t0 + 1 < t1 ? look(t0 + 1) : 0;
+            if (t0 + 2 < t1) next = look(t0 + 2);
+            hand_on(t0, a);
+            if (t0 + 1 < t1) hand_on(t0 + 1, b);
+        }
         __syncthreads();
-        u64 nbad = 0;
-        if (more) {
-            nbad = __ballot(next >= p.c.cap);
-            fetch(next < p.c.cap ? next : 0);
-            if (t + 2 < t1) next = look(t + 2);
+        fetch(t0);
+        store(t0);
+    }
+#pragma unroll 1
+    for (u32 t = t0; t < t1; t++) {
+        const u32 kt = tiles.key(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if (wave == 0 && t + 2 < t1) {
+            hand_on(t + 2, next);
+            if (t + 3 < t1) next = look(t + 3);
         }
         if (live && span.any(kt, KT)) {
+            const u32 buf = (t - t0) & 1;
+            u32 ii = i;
+            asm volatile("" : "+v"(ii));
             const char *const kp = s_k + buf * (W::PL * W::KP), *const vp = s_v + buf * (W::PL * W::VP);
+            const u32 krd = W::kat((ii & 19) | ((ii & 4) << 1) | ((ii & 8) >> 1), h), vrd = W::vat(ii, h);
 #pragma unroll
             for (int sub = 0; sub < KT / 32; sub++) {
                 const u32 kb = kt + 32 * sub;
                 f16_t s;
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[e] = 0.f;
+                {
+                    h8_t a[CK_AHEAD], b[CK_AHEAD];
+                    auto read = [&](int j) {
+                        const char *at = kp + W::kput(krd, W::kat(32 * sub, 2 * j));
+                        a[j % CK_AHEAD] = *(const h8_t *)at;
+                        if constexpr (Q8) b[j % CK_AHEAD] = *(const h8_t *)(at + W::KP);
+                    };
 #pragma unroll
-                for (int j = 0; j < NS; j++) {
-                    const char *at = kp + W::kput(krd, W::kat(32 * sub, 2 * j));
-                    const h8_t a = *(const h8_t *)at;
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[j], s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[j], s, 0, 0, 0);
-                    if constexpr (Q8) {
-                        const h8_t b = *(const h8_t *)(at + (W::PL - 1) * W::KP);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, qh[j], s, 0, 0, 0);
+                    for (int j = 0; j < CK_AHEAD; j++) read(j);
+#pragma unroll
+                    for (int j = 0; j < NS; j++) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % CK_AHEAD], qh[j], s, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % CK_AHEAD], ql[j], s, 0, 0, 0);
+                        if constexpr (Q8) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[j % CK_AHEAD], qh[j], s, 0, 0, 0);
+                        if (j + CK_AHEAD < NS) read(j + CK_AHEAD);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if constexpr (BIAS) {
 #pragma unroll
                     for (int e = 0; e < 16; e++)
                         s[e] = ck_score<true>(s[e], cs, p.softcap, icap, slope, pq, kb + 16 * (e >> 3) + 8 * h + (e & 7));
                 }
-                const u32 mybad = (u32)(bad >> (32 * sub));
-                if (!span.full(kb, 32) || mybad) {
-                    const u32 odd = (u32)((s_odd[buf][0] | s_odd[buf][1]) >> (32 * sub));
+                const u32 bad = (u32)(s_bad[(t - t0) & 3] >> (32 * sub));
+                if (!span.full(kb, 32) || bad) {
+                    const u32 odd = (u32)((Q8 ? s_odd[buf][2] | s_odd[buf][3]
+                                              : s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3]) >> (32 * sub));
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
-                        const bool v = see.sees(kb + k) && !((mybad >> k) & 1);
+                        const bool v = see.sees(kb + k) && !((bad >> k) & 1);
                         s[e] = v ? s[e] : -INFINITY;
                         if (v && ((odd >> k) & 1)) l = NAN;
                     }
@@ -633,38 +687,50 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                     m = mn;
                 }
                 const float mref = m == -INFINITY ? 0.f : m - CK_UP;
-                h8_t ph[2], pl[2];
+                h8_t v[CK_AHEAD], w[CK_AHEAD];
+                auto read = [&](int j) {
+                    const char *at = vp + W::vput(vrd, W::vat(32 * (j % NO), 4 * sub + 2 * (j / NO)));
+                    v[j % CK_AHEAD] = *(const h8_t *)at;
+                    if constexpr (Q8) w[j % CK_AHEAD] = *(const h8_t *)(at + W::VP);
+                };
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float pe = __builtin_amdgcn_exp2f(BIAS ? s[e] - mref : fmaf(s[e], cs, -mref));
-                    l += pe;
-                    _Float16 a, b;
-                    ck_split(pe, a, b);
-                    ph[e >> 3][e & 7] = a;
-                    pl[e >> 3][e & 7] = b;
+                for (int j = 0; j < CK_AHEAD && j < 2 * NO; j++) read(j);
+                __builtin_amdgcn_sched_barrier(0);
+                u4_t ph[2], pl[2];
+                float l1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float a = __builtin_amdgcn_exp2f(BIAS ? s[e] - mref : fmaf(s[e], cs, -mref));
+                    const float b = __builtin_amdgcn_exp2f(BIAS ? s[e + 1] - mref : fmaf(s[e + 1], cs, -mref));
+                    l += a;
+                    l1 += b;
+                    u32 hi, lo;
+                    ck_split2(a, b, hi, lo);
+                    ph[e >> 3][(e & 7) >> 1] = hi;
+                    pl[e >> 3][(e & 7) >> 1] = lo;
                 }
+                l += l1;
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int b = 0; b < NO; b++) {
-                        const char *at = vp + W::vput(vrd, W::vat(32 * b, 4 * sub + 2 * u));
-                        const h8_t v = *(const h8_t *)at;
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u], o[b], 0, 0, 0);
-                        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u], o[b], 0, 0, 0);
-                        if constexpr (Q8) {
-                            const h8_t w = *(const h8_t *)(at + (W::PL - 1) * W::VP);
-                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ph[u], o[b], 0, 0, 0);
-                        }
-                    }
+                for (int j = 0; j < 2 * NO; j++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int b = j % NO, u = j / NO;
+                    const h8_t x = __builtin_bit_cast(h8_t, ph[u]), y = __builtin_bit_cast(h8_t, pl[u]);
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % CK_AHEAD], x, o[b], 0, 0, 0);
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % CK_AHEAD], y, o[b], 0, 0, 0);
+                    if constexpr (Q8) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[j % CK_AHEAD], x, o[b], 0, 0, 0);
+                    if (j + CK_AHEAD < 2 * NO) read(j + CK_AHEAD);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (more) store(buf ^ 1, nbad, nbad || !all.full(tiles.key(t + 1), KT));
-        bad = nbad;
+        if (t + 1 < t1) store(t + 1);
     }
     l += __shfl_xor(l, 32);
     if (!live || cw + i >= cols) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (sq.ns == 1) {
+        const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+        const u64 brow = (u64)sq.row + r;
         float *d = p.dst + brow * p.q_stride + (u64)head * D + 4 * h;
 #pragma unroll
         for (int b = 0; b < NO; b++)
