@@ -591,3 +591,31 @@ def test_prompt_evict_decode(T, q8):
         skip[i] += lens[i] - keeps[i]
     for k in range(3):
         step([(17 + k, 1), (26 + k, 1)])
+
+
+def test_kv_evict_captured(T):
+    """A captured eviction (which takes no workspace) replays to the eager call's result, short
+    and long, also with eager evictions on the same stream between."""
+    import tlkv
+    rng = np.random.default_rng(3)
+    lens, keeps = [700, 30000], [300, 12000]
+    w = [T.from_numpy(np.round(rng.standard_normal(n) * 8).astype(np.float32)).cuda() for n in lens]
+    kept = [T.zeros(k, dtype=T.int32, device="cuda") for k in keeps]
+    seqs = (tlkv.EvictSeq * 2)(*[
+        tlkv.EvictSeq(weight=w[i].data_ptr(), len=lens[i], keep=keeps[i], sink=1, recent=9, page_size=1,
+                      kept=kept[i].data_ptr()) for i in (0, 1)])
+    s = T.cuda.Stream()
+    h = tlkv.stream_handle(s)
+    T.cuda.synchronize()
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g, stream=s):
+        tlkv.check(tlkv.lib().tl_kv_evict(seqs, 2, h))
+    want = [R.evict(x.cpu().numpy(), n, k, 1, 9)[0] for x, n, k in zip(w, lens, keeps)]
+    for _ in range(3):
+        for run in (g.replay, lambda: tlkv.check(tlkv.lib().tl_kv_evict(seqs, 2, h))):
+            for x in kept:
+                x.zero_()
+            T.cuda.synchronize()
+            run()
+            T.cuda.synchronize()
+            assert all(np.array_equal(x.cpu().numpy(), y) for x, y in zip(kept, want))

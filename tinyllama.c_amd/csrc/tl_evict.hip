@@ -9,32 +9,305 @@
 #define EV_MAX_SEQ 16
 #define EV_THREADS 1024
 #define EV_WAVES (EV_THREADS / 64)
+#define EV_ONE 8                            /* keys of a thread where one workgroup has a session */
+#define EV_PER 2                            /* ... where several share it: more of them run at once */
+#define EV_SEG (EV_THREADS * EV_PER)        /* positions of one of these */
+#define EV_BINS 2048                        /* digits of 11, 11 and 10 bits */
+#define EV_LOW 1024
+#define EV_MAX_SEG EV_THREADS               /* segments of a session that several workgroups share */
+#define EV_CNT (2 * EV_BINS + EV_LOW)       /* their histograms, zero between calls */
+#define EV_SEGW (EV_LOW + 8)                /* scratch words of a segment: counts by the last digit */
+static_assert(EV_MAX_SEQ * EV_CNT <= TL_MERGE_MAX_GROUPS * TL_MERGE_PAD, "counters of a stream's workspace");
 
 struct EvSeq {
     const float *w;
     const u32 *pages;
     u32 *kept, *rows, *freed;
     float *w_out;
-    u32 len, keep, sink, recent, shift;
+    u32 *cnt;                               /* EV_CNT words, zero between calls */
+    u32 *seg;                               /* EV_SEGW words per segment */
+    u32 len, keep, sink, recent, shift, wg0;
 };
 struct EvParams {
     EvSeq seq[EV_MAX_SEQ];
+    u32 n_seq;
 };
 
 /* order of the weights as unsigned numbers: NaN lowest, -0 as 0; positions
  * that stay in any case highest */
-TL_DEV u32 ev_key(const EvSeq &s, u32 j) {
+TL_DEV u32 ev_order(const EvSeq &s, u32 j, float w) {
     if (j < s.sink || j >= s.len - s.recent) return 0xffffffffu;
-    const float w = s.w[j];
     if (w != w) return 0;
     const u32 b = __float_as_uint(w + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+TL_DEV u32 ev_key(const EvSeq &s, u32 j) { return ev_order(s, j, s.w[j]); }
 
-/* One workgroup per session.  Radix select of the keep-th largest key (four
- * passes of 8 bits, histograms in LDS), then one pass in position order that
- * ranks the kept and the evicted positions: of the keys equal to the
- * threshold the first ones stay. */
+/* inclusive sum over the wave's lanes: DPP moves within rows of 16, then the
+ * rows' last lanes broadcast */
+TL_DEV u32 ev_wave_scan(u32 x) {
+#define EV_STEP(ctrl, rows) x += (u32)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+    EV_STEP(0x111, 0xf);
+    EV_STEP(0x112, 0xf);
+    EV_STEP(0x114, 0xf);
+    EV_STEP(0x118, 0xf);
+    EV_STEP(0x142, 0xa);
+    EV_STEP(0x143, 0xc);
+#undef EV_STEP
+    return x;
+}
+
+/* Exclusive sum over the workgroup's threads, and the total.  One barrier: the
+ * caller has one of its own between a scan and the next use of s_w. */
+TL_DEV u32 ev_scan(u32 x, u32 *s_w, u32 &total) {
+    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const u32 y = ev_wave_scan(x);
+    if (lane == 63) s_w[wave] = y;
+    __syncthreads();
+    u32 base = 0;
+    total = 0;
+#pragma unroll
+    for (u32 w = 0; w < EV_WAVES; w++) {
+        base += w < wave ? s_w[w] : 0;
+        total += s_w[w];
+    }
+    return base + y - x;
+}
+
+/* The bin that holds the want-th key from the top, its rank in there and the
+ * bin's keys; h: the thread's bins, 2047 - 2 tid downwards (a histogram of 1024
+ * bins: the lowest of them).  Two barriers. */
+TL_DEV void ev_pick(u32 h0, u32 h1, u32 &want, u32 &bin, u32 &held, u32 *s_w, u32 *s_pick) {
+    u32 total;
+    const u32 at = ev_scan(h0 + h1, s_w, total), tid = threadIdx.x;
+    if (at < want && want <= at + h0) {
+        s_pick[0] = EV_BINS - 1 - 2 * tid;
+        s_pick[1] = want - at;
+        s_pick[2] = h0;
+    } else if (at + h0 < want && want <= at + h0 + h1) {
+        s_pick[0] = EV_BINS - 2 - 2 * tid;
+        s_pick[1] = want - at - h0;
+        s_pick[2] = h1;
+    }
+    __syncthreads();
+    bin = s_pick[0];
+    want = s_pick[1];
+    held = s_pick[2];
+}
+/* the thread's two bins of a histogram of n (2048 or 1024) */
+template <u32 N>
+TL_DEV uint2 ev_bins(const u32 *h) {
+    if (2 * threadIdx.x < EV_BINS - N) return make_uint2(0, 0);
+    const uint2 v = *(const uint2 *)&h[EV_BINS - 2 - 2 * threadIdx.x];
+    return make_uint2(v.y, v.x);
+}
+
+/* Writes the workgroup's positions j0 .. (the thread has PER of them, keys k):
+ * keys above `top` stay, and of those equal to it the first `want` of the
+ * session (all of them if `all`); kept / equal: how many the positions before
+ * the workgroup's have of them.  The order goes through LDS, so that
+ * neighbouring threads write neighbouring words. */
+template <u32 PER>
+TL_DEV void ev_write(const EvSeq &s, u32 j0, const u32 (&k)[PER], u32 top, u32 want, bool all, u32 kept, u32 equal,
+                     u32 *s_w, u16 *s_at) {
+    const u32 n = min(s.len - j0, PER * EV_THREADS), p0 = threadIdx.x * PER;
+    u32 total;
+    if (!all) {
+        u32 eq = 0;
+#pragma unroll
+        for (u32 e = 0; e < PER; e++) eq += p0 + e < n && k[e] == top;
+        equal += ev_scan(eq, s_w, total);
+        __syncthreads();
+    }
+    u32 stay = 0;
+#pragma unroll
+    for (u32 e = 0; e < PER; e++) {
+        const bool is = p0 + e < n && k[e] == top;
+        stay |= (u32)(p0 + e < n && (k[e] > top || (is && (all || equal < want)))) << e;
+        equal += is;
+    }
+    u32 at = ev_scan((u32)__popc(stay), s_w, total);
+#pragma unroll
+    for (u32 e = 0; e < PER; e++) {
+        const bool is = (stay >> e) & 1;
+        if (p0 + e < n) s_at[is ? at : total + (p0 + e - at)] = (u16)(p0 + e);
+        at += is;
+    }
+    __syncthreads();
+    /* all the look-ups requested before the first is used */
+    u32 j[PER], row[PER];
+    float w[PER];
+#pragma unroll
+    for (u32 e = 0; e < PER; e++) {
+        const u32 x = min(threadIdx.x + e * EV_THREADS, n - 1);
+        j[e] = j0 + s_at[x];
+        row[e] = s.pages ? s.pages[j[e] >> s.shift] : j[e] >> s.shift;
+        w[e] = s.w_out ? s.w[j[e]] : 0.f;
+    }
+#pragma unroll
+    for (u32 e = 0; e < PER; e++) {
+        const u32 x = threadIdx.x + e * EV_THREADS;
+        const u32 r = (row[e] << s.shift) + (j[e] & ((1u << s.shift) - 1));
+        if (x >= n) break;
+        if (x < total) {
+            if (s.kept) s.kept[kept + x] = j[e];
+            if (s.rows) s.rows[kept + x] = r;
+            if (s.w_out) s.w_out[kept + x] = w[e];
+        } else if (s.freed) {
+            s.freed[j0 - kept + (x - total)] = r;
+        }
+    }
+}
+
+/* digit d of a key, and whether the digits before it are `pref` */
+TL_DEV u32 ev_digit(u32 k, int d) { return d == 0 ? k >> 21 : d == 1 ? (k >> 10) & (EV_BINS - 1) : k & (EV_LOW - 1); }
+TL_DEV bool ev_under(u32 k, int d, u32 pref) { return d == 0 || k >> (d == 1 ? 21 : 10) == pref; }
+TL_DEV u32 ev_join(u32 pref, int d, u32 bin) { return d == 0 ? bin : (pref << (d == 1 ? 11 : 10)) | bin; }
+
+/* A session of at most 8192 positions: one workgroup, the keys in registers,
+ * the keep-th largest by three digits whose histograms lie in LDS.  Bound by
+ * the chain of barriers and round trips. */
+__global__ __launch_bounds__(EV_THREADS) void evict_one_kernel(const EvParams p) {
+    __shared__ __align__(8) u32 s_hist[EV_BINS];
+    __shared__ u32 s_w[EV_WAVES], s_pick[3];
+    __shared__ u16 s_at[EV_ONE * EV_THREADS];
+    const EvSeq &s = p.seq[blockIdx.x];
+    const u32 tid = threadIdx.x, j0 = tid * EV_ONE;
+    float w[EV_ONE];
+    u32 k[EV_ONE];
+#pragma unroll
+    for (u32 e = 0; e < EV_ONE; e++) w[e] = s.w[min(j0 + e, s.len - 1)];    /* all requested at once */
+    *(uint2 *)&s_hist[2 * tid] = make_uint2(0, 0);
+#pragma unroll
+    for (u32 e = 0; e < EV_ONE; e++) k[e] = ev_order(s, j0 + e, w[e]);
+    __syncthreads();
+    u32 want = s.keep, pref = 0, held = 0;
+#pragma unroll
+    for (int d = 0; d < 3; d++) {
+#pragma unroll
+        for (u32 e = 0; e < EV_ONE; e++)
+            if (j0 + e < s.len && ev_under(k[e], d, pref)) atomicAdd(&s_hist[ev_digit(k[e], d)], 1u);
+        __syncthreads();
+        const uint2 h = ev_bins<EV_BINS>(s_hist);
+        *(uint2 *)&s_hist[EV_BINS - 2 - 2 * tid] = make_uint2(0, 0);
+        u32 bin;
+        ev_pick(h.x, h.y, want, bin, held, s_w, s_pick);
+        pref = ev_join(pref, d, bin);
+    }
+    ev_write(s, 0, k, pref, want, want == held, 0, 0, s_w, s_at);
+}
+
+TL_DEV const EvSeq &ev_mine(const EvParams &p) {
+    u32 i = 0;
+    while (i + 1 < p.n_seq && p.seq[i + 1].wg0 <= blockIdx.x) i++;
+    return p.seq[i];
+}
+
+/* the digits before DIGIT from the session's histograms, by every workgroup for itself */
+template <int DIGIT>
+TL_DEV u32 ev_prefix(const EvSeq &s, u32 &want, u32 &held, u32 *s_w, u32 *s_pick) {
+    uint2 h[3];
+    u32 pref = 0;
+    if constexpr (DIGIT > 0) h[0] = ev_bins<EV_BINS>(s.cnt);
+    if constexpr (DIGIT > 1) h[1] = ev_bins<EV_BINS>(s.cnt + EV_BINS);
+    if constexpr (DIGIT > 2) h[2] = ev_bins<EV_LOW>(s.cnt + 2 * EV_BINS);
+    want = s.keep;
+#pragma unroll
+    for (int d = 0; d < DIGIT; d++) {
+        u32 bin;
+        ev_pick(h[d].x, h[d].y, want, bin, held, s_w, s_pick);
+        pref = ev_join(pref, d, bin);
+    }
+    return pref;
+}
+
+/* Longer sessions: a workgroup per EV_SEG positions, one launch per digit.  A
+ * workgroup adds its LDS histogram to the session's (integer atomics); those of
+ * the next launch find the digit from it, each for itself (one round trip with
+ * their keys'; a last workgroup that did it for all cost three more: 43 us for
+ * 131072 positions).  The last digit's counts are also kept by segment. */
+template <int DIGIT>
+__global__ __launch_bounds__(EV_THREADS) void evict_digit_kernel(const EvParams p) {
+    constexpr u32 NB = DIGIT == 2 ? EV_LOW : EV_BINS;
+    __shared__ __align__(8) u32 s_hist[EV_BINS];
+    __shared__ u32 s_w[EV_WAVES], s_pick[3];
+    const EvSeq &s = ev_mine(p);
+    const u32 seg = blockIdx.x - s.wg0, tid = threadIdx.x;
+    float w[EV_PER];
+    u32 k[EV_PER];
+#pragma unroll
+    for (u32 e = 0; e < EV_PER; e++) w[e] = s.w[min(seg * EV_SEG + e * EV_THREADS + tid, s.len - 1)];
+    *(uint2 *)&s_hist[2 * tid] = make_uint2(0, 0);
+    u32 want, held;
+    const u32 pref = ev_prefix<DIGIT>(s, want, held, s_w, s_pick);
+    __syncthreads();
+    u32 above = 0;
+#pragma unroll
+    for (u32 e = 0; e < EV_PER; e++) {
+        const u32 j = seg * EV_SEG + e * EV_THREADS + tid;
+        k[e] = ev_order(s, j, w[e]);
+        if (j >= s.len) continue;
+        if (ev_under(k[e], DIGIT, pref)) atomicAdd(&s_hist[ev_digit(k[e], DIGIT)], 1u);
+        above += DIGIT == 2 && k[e] >> 10 > pref;
+    }
+    __syncthreads();
+    u32 *hist = s.cnt + DIGIT * EV_BINS;
+#pragma unroll
+    for (u32 e = 0; e < NB / EV_THREADS; e++) {
+        const u32 n = s_hist[e * EV_THREADS + tid];
+        if (n) __hip_atomic_fetch_add(&hist[e * EV_THREADS + tid], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if constexpr (DIGIT == 2) {
+        /* word d: the segment's keys with a digit of d or more, or above pref (1024: these alone) */
+        u32 *sw = s.seg + (u64)seg * EV_SEGW;
+        u32 total, all;
+        ev_scan(above, s_w, total);
+        __syncthreads();
+        const u32 n = s_hist[NB - 1 - tid];
+        const u32 over = total + ev_scan(n, s_w, all);
+        sw[NB - 1 - tid] = over + n;
+        if (tid == 0) sw[NB] = total;
+    }
+}
+
+__global__ __launch_bounds__(EV_THREADS) void evict_write_kernel(const EvParams p) {
+    __shared__ u32 s_w[EV_WAVES], s_pick[3], s_base[2];
+    __shared__ u16 s_at[EV_SEG];
+    const EvSeq &s = ev_mine(p);
+    const u32 tid = threadIdx.x, seg = blockIdx.x - s.wg0, j0 = seg * EV_SEG, p0 = j0 + tid * EV_PER;
+    u32 k[EV_PER];
+    float w[EV_PER];
+#pragma unroll
+    for (u32 e = 0; e < EV_PER; e++) w[e] = s.w[min(p0 + e, s.len - 1)];
+#pragma unroll
+    for (u32 e = 0; e < EV_PER; e++) k[e] = ev_order(s, p0 + e, w[e]);
+    u32 want, held, total;
+    const u32 top = ev_prefix<3>(s, want, held, s_w, s_pick);
+    /* what the segments before this one hold: a thread each (at most EV_MAX_SEG) */
+    const u32 bin = top & (EV_LOW - 1);
+    const u32 *sw = s.seg + (u64)tid * EV_SEGW + bin;
+    const u32 more = tid < seg ? sw[1] : 0, eq = tid < seg ? sw[0] - more : 0;
+    __syncthreads();
+    const u32 eq0 = ev_scan(eq, s_w, total);
+    if (tid == 0) s_base[0] = total;
+    const u32 stay = more + (eq0 < want ? min(eq, want - eq0) : 0);
+    __syncthreads();
+    ev_scan(stay, s_w, total);
+    if (tid == 0) s_base[1] = total;
+    __syncthreads();
+    ev_write(s, j0, k, top, want, want == held, s_base[1], s_base[0], s_w, s_at);
+}
+
+/* the histograms back to zero, once the last launch that reads them is through */
+__global__ __launch_bounds__(EV_THREADS) void evict_clear_kernel(const EvParams p) {
+    for (u32 x = threadIdx.x; x < EV_CNT; x += EV_THREADS) p.seq[blockIdx.x].cnt[x] = 0;
+}
+
+/* Any length without a workspace (captured calls, sessions past EV_MAX_SEG
+ * segments): one workgroup per session.  Radix select of the keep-th largest
+ * key (four passes of 8 bits, histograms in LDS), then one pass in position
+ * order that ranks the kept and the evicted positions: of the keys equal to
+ * the threshold the first ones stay. */
 __global__ __launch_bounds__(EV_THREADS) void evict_kernel(const EvParams p) {
     __shared__ u32 s_hist[256];
     __shared__ u32 s_want, s_pref;
@@ -124,27 +397,60 @@ extern "C" int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *strea
                     return tl_fail(TL_EINVAL, "evict: session %u: outputs overlap", i);
         }
     }
-    for (u32 i = 0; i < n_seq; i += EV_MAX_SEQ) {
-        const u32 m = n_seq - i < EV_MAX_SEQ ? n_seq - i : EV_MAX_SEQ;
-        EvParams p;
-        memset(&p, 0, sizeof(p));
-        for (u32 j = 0; j < m; j++) {
-            const tl_evict_seq &q = seqs[i + j];
-            EvSeq &s = p.seq[j];
-            s.w = q.weight;
-            s.pages = q.pages;
-            s.kept = q.kept;
-            s.rows = q.rows;
-            s.freed = q.freed;
-            s.w_out = q.weight_out;
-            s.len = q.len;
-            s.keep = q.keep;
-            s.sink = q.sink;
-            s.recent = q.recent;
-            s.shift = (u32)__builtin_ctz(q.page_size);
+    const hipStream_t st = (hipStream_t)stream;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    bool asked = false;
+    /* three kinds of sessions: one workgroup's registers, several workgroups, neither */
+    for (int kind = 0; kind < 3; kind++) {
+        for (u32 i = 0; i < n_seq;) {
+            EvParams p;
+            memset(&p, 0, sizeof(p));
+            u32 wgs = 0;
+            for (; i < n_seq && p.n_seq < EV_MAX_SEQ; i++) {
+                const tl_evict_seq &q = seqs[i];
+                int mine = 0;
+                if (q.len > EV_ONE * EV_THREADS) {
+                    if (!asked) HIP_TRY(hipStreamIsCapturing(st, &cap));
+                    asked = true;
+                    mine = cap == hipStreamCaptureStatusNone && q.len <= EV_SEG * EV_MAX_SEG ? 1 : 2;
+                }
+                if (mine != kind) continue;
+                EvSeq &s = p.seq[p.n_seq++];
+                s.w = q.weight;
+                s.pages = q.pages;
+                s.kept = q.kept;
+                s.rows = q.rows;
+                s.freed = q.freed;
+                s.w_out = q.weight_out;
+                s.len = q.len;
+                s.keep = q.keep;
+                s.sink = q.sink;
+                s.recent = q.recent;
+                s.shift = (u32)__builtin_ctz(q.page_size);
+                s.wg0 = wgs;
+                wgs += kind == 1 ? (q.len + EV_SEG - 1) / EV_SEG : 1;
+            }
+            if (!p.n_seq) break;
+            if (kind == 0) {
+                hipLaunchKernelGGL(evict_one_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+            } else if (kind == 2) {
+                hipLaunchKernelGGL(evict_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+            } else {
+                TlWorkspace *w;
+                const int rc = tl_workspace_get(st, (size_t)wgs * EV_SEGW, 0, TL_MERGE_CNT_WORDS, &w);
+                if (rc) return rc;
+                for (u32 j = 0; j < p.n_seq; j++) {
+                    p.seq[j].cnt = w->cnt + (size_t)j * EV_CNT;
+                    p.seq[j].seg = (u32 *)w->acc + (size_t)p.seq[j].wg0 * EV_SEGW;
+                }
+                hipLaunchKernelGGL(evict_digit_kernel<0>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+                hipLaunchKernelGGL(evict_digit_kernel<1>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+                hipLaunchKernelGGL(evict_digit_kernel<2>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+                hipLaunchKernelGGL(evict_write_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
+                hipLaunchKernelGGL(evict_clear_kernel, dim3(p.n_seq), dim3(EV_THREADS), 0, st, p);
+            }
+            HIP_TRY(hipGetLastError());
         }
-        hipLaunchKernelGGL(evict_kernel, dim3(m), dim3(EV_THREADS), 0, (hipStream_t)stream, p);
-        HIP_TRY(hipGetLastError());
     }
     return TL_OK;
 }
