@@ -9,6 +9,7 @@
 #define CK_KEYS 32             /* keys of one tile */
 #define CK_COLS 16             /* (row, head) columns of a narrow workgroup */
 #define CK_WCOLS 128           /* ... of a wide one */
+#define CK_WKEYS 256           /* keys of a wide workgroup of the attention weight */
 
 /* Split merge: one arrival counter per group, zero between launches, at the
  * start of the workspace; (max, sum) pairs and partial rows follow. */
@@ -80,18 +81,41 @@ TL_DEV u32 ck_find(const u32 *wg0, u32 n_seq, u32 b) {
     return (u32)__builtin_amdgcn_readfirstlane((int)__popc((u32)__ballot(wg0[lane] <= b)) - 1);
 }
 
-/* exp(2|x|) based above 1/4 ((e - 1) / (e + 1): the subtraction is exact to
- * the rounding of e), the odd series below, so the result is good to a few
- * units of its last place over the whole range */
-TL_DEV float ck_tanh(float x) {
-    const float ax = fabsf(x), x2 = x * x;
-    const float e = __builtin_amdgcn_exp2f(fminf(ax, 10.f) * (2.f * CK_LOG2E));
-    const float big = copysignf((e - 1.f) * __builtin_amdgcn_rcpf(e + 1.f), x);
-    float s = fmaf(x2, 62.f / 2835.f, -17.f / 315.f);
-    s = fmaf(x2, s, 2.f / 15.f);
-    s = fmaf(x2, s, -1.f / 3.f);
-    const float small = fmaf(x * x2, s, x);
-    return ax < 0.25f ? small : big;
+/* tanh of N scores x c.  Below 0.6 a polynomial (odd, five coefficients fitted
+ * to a relative error of 3e-9): scores lie far below their cap as a rule, and
+ * there the error of the capped score has to be relative to the score, not to
+ * the cap.  Where one of the wave's is above, (e - 1) / (e + 1) from e = exp(2
+ * x) for those (its error, 1e-7 of the cap, is relative there). */
+template <int N, class T>
+TL_DEV void ck_tanh(T &s, float c) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        s[e] *= c;
+        top = fmaxf(top, fabsf(s[e]));
+    }
+    const bool big = __any(top >= 0.6f);
+    float t[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        const float x = s[e], z = x * x;
+        float q = fmaf(z, -0.005895147565752268f, 0.02079596184194088f);
+        q = fmaf(z, q, -0.053783826529979706f);
+        q = fmaf(z, q, 0.13331924378871918f);
+        q = fmaf(z, q, -0.33333298563957214f);
+        t[e] = fmaf(x * z, q, x);
+    }
+    if (big) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float x = s[e] > 20.f ? 20.f : s[e];
+            const float y = __builtin_amdgcn_exp2f(x * (2.f * CK_LOG2E));
+            const float u = (y - 1.f) * __builtin_amdgcn_rcpf(y + 1.f);
+            t[e] = fabsf(x) < 0.6f ? t[e] : u;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) s[e] = t[e];
 }
 
 /* two f32 as pairs of f16 whose sums have 22 bits of them (x - hi is exact, one
@@ -126,6 +150,7 @@ struct CkSees {
     TL_DEV bool sees(u32 key) const { return key - lo < w || key - f < pw; }
 };
 
+/* over N neighbouring lanes */
 template <int N>
 TL_DEV u32 group_umin(u32 x) {
 #pragma unroll
@@ -146,20 +171,21 @@ TL_DEV u32 group_umax(u32 x) {
 }
 TL_DEV u32 ck_uniform(u32 x) { return (u32)__builtin_amdgcn_readfirstlane((int)x); }
 
-/* What a block of columns sees together: the lowest and highest keys of its
- * causal part and of its prefix, and the range that every column sees. */
+/* What the columns of rows r0 .. r1 (positions p0 .. p1) see together: from the
+ * positions alone, and from the range of their first positions where rows have
+ * those. */
 struct CkSpan {
     u32 fmin, lo, hi, max_lo, min_hi, max_f, pre;
-    /* N: lanes over which the columns lie (the other lanes repeat them) */
-    template <int N>
-    TL_DEV void set(const CkSees &s) {
-        fmin = ck_uniform(group_umin<N>(s.pw ? s.f : ~0u));
-        lo = ck_uniform(group_umin<N>(s.w ? s.lo : ~0u));
-        hi = ck_uniform(group_umax<N>(s.w ? s.hi : 0));
-        max_lo = ck_uniform(group_umax<N>(s.lo));
-        min_hi = ck_uniform(group_umin<N>(s.hi));
-        max_f = ck_uniform(group_umax<N>(s.f));
-        pre = ck_uniform(s.pre);
+    TL_DEV void set(u32 p0, u32 p1, u32 end, u32 window, u32 prefix, u32 first_min, u32 first_max) {
+        fmin = first_min;
+        max_f = first_max;
+        pre = prefix < end ? prefix : end;
+        lo = window && p0 + 1 > window ? p0 + 1 - window : 0;
+        lo = lo > fmin ? lo : fmin;
+        hi = p1 + 1;
+        max_lo = window && p1 + 1 > window ? p1 + 1 - window : 0;
+        max_lo = max_lo > max_f ? max_lo : max_f;
+        min_hi = p0 + 1;
     }
     /* every column sees every one of the n keys from kb on */
     TL_DEV bool full(u32 kb, u32 n) const {
@@ -178,11 +204,11 @@ struct CkTiles {
     u32 a0, na, b0, nb;
     TL_DEV void set(const CkSpan &s) {
         a0 = na = b0 = nb = 0;
-        if (s.fmin != ~0u) {
+        if (s.fmin < s.pre) {
             a0 = s.fmin / KT;
             na = (s.pre + KT - 1) / KT - a0;
         }
-        if (s.lo != ~0u) {
+        if (s.lo < s.hi) {
             b0 = s.lo / KT;
             const u32 b1 = (s.hi + KT - 1) / KT;
             if (na && b0 < a0 + na) b0 = a0 + na;
@@ -403,14 +429,37 @@ TL_DEV float ck_split_q(const float4 (&x)[D / (8 * G)][2], float scale, h8_t (&h
     return down * scale;
 }
 
-/* the eight scores of a lane from its products, in units of log2 */
+/* How products become scores in units of log2: s * mul after apply(). */
 template <bool BIAS>
-TL_DEV float ck_score(float s, float cs, float softcap, float icap, float slope, u32 p, u32 key) {
-    float x = s * cs;
-    if constexpr (BIAS) {
-        if (softcap > 0.f) x = softcap * ck_tanh(x * icap);
-        x = fmaf(-slope, (float)(p > key ? p - key : key - p), x);
-        x *= CK_LOG2E;
+struct CkScore {
+    float mul, cap_in, slope, softcap;
+    bool capped, sloped;
+    /* cs: factor from the products to scale * q.k */
+    TL_DEV void set(const CkAttnParams &p, float cs, u32 head) {
+        mul = cs * CK_LOG2E;
+        if constexpr (BIAS) {
+            capped = p.softcap > 0.f;
+            sloped = p.slopes != nullptr;
+            slope = sloped ? p.slopes[head] * CK_LOG2E : 0.f;
+            softcap = p.softcap;
+            finish(cs);
+        }
     }
-    return x;
-}
+    TL_DEV void finish(float cs) {
+        mul = capped ? softcap * CK_LOG2E : cs * CK_LOG2E;
+        cap_in = capped ? cs / softcap : 0.f;
+    }
+    /* far0: position minus the key of element 0; off(e): how far key e lies behind that */
+    template <int N, class T, class F>
+    TL_DEV void apply(T &s, int far0, F off) const {
+        if constexpr (BIAS) {
+            if (capped) ck_tanh<N>(s, cap_in);
+            if (sloped) {
+                const float f = (float)far0;
+#pragma unroll
+                for (int e = 0; e < N; e++) s[e] = fmaf(s[e], mul, -slope * fabsf(f - (float)off(e)));
+            }
+        }
+    }
+    TL_DEV float factor() const { return BIAS && sloped ? 1.f : mul; }
+};

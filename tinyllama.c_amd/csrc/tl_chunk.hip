@@ -430,7 +430,7 @@ static u32 next_chunks(const tl_chunk *ch, u32 n_chunk, u32 *at, const tl_chunk 
     return m;
 }
 
-/* most partial rows that the launches of one group of chunks take */
+/* most partial rows that the attention's launches of one group of chunks take */
 static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, u32 window, const tl_chunk *ch, u32 n_chunk,
                        u64 *parts) {
     AttnPlan pl;
@@ -445,30 +445,98 @@ static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, u32 window, const tl_chu
     return true;
 }
 
+/* The attention weight's launches of one group of chunks: [0] few columns, [1]
+ * many, whose sums take `floats` of workspace. */
+struct WeightPlan {
+    CkSeq seq[2][CK_MAX_SEQ];
+    u32 n[2], wgs[2], blocks;
+    u64 floats;
+};
+
+/* More columns than this keep 256 keys of one head to a workgroup; fewer go
+ * through all heads of 32 keys, where reading K is the work. */
+#define CK_WEIGHT_WIDE_MIN 32
+
+static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 window) {
+    pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.blocks = 0;
+    pl.floats = 0;
+    u64 wgs[2] = {0, 0}, blocks = 0, shares = 0;
+    for (u32 i = 0; i < n; i++) {
+        const u64 cols = (u64)ch[i]->n * gqa, end = (u64)ch[i]->pos + ch[i]->n;
+        const int w = cols > CK_WEIGHT_WIDE_MIN;
+        CkSeq &s = pl.seq[w][pl.n[w]++];
+        seq_of(s, *ch[i]);
+        /* first key that a window leaves (documents' starts are known on the device only) */
+        u64 lo = window && (u64)ch[i]->pos + 1 > window && !ch[i]->prefix ? (u64)ch[i]->pos + 1 - window : 0;
+        if (!w) {
+            s.ncb = (u32)((cols + CK_COLS - 1) / CK_COLS);
+            s.part0 = (u32)(lo / CK_KEYS * CK_KEYS);
+            s.wg0 = (u32)wgs[0];
+            wgs[0] += (end - s.part0 + CK_KEYS - 1) / CK_KEYS;
+        } else {
+            s.part0 = (u32)(lo / CK_WKEYS * CK_WKEYS);
+            s.ncb = (u32)((end - s.part0 + CK_WKEYS - 1) / CK_WKEYS);
+            blocks += s.ncb;
+            shares += (u64)s.ncb * ((cols + 127) / 128);
+        }
+    }
+    /* shares of 128 columns at least, two workgroups to a CU */
+    const u64 per = (shares * n_kv + 511) / 512;
+    for (u32 i = 0; i < pl.n[1]; i++) {
+        CkSeq &s = pl.seq[1][i];
+        const u64 parts = ((u64)s.n * gqa + 127) / 128;
+        s.ns = (u32)(per > 1 ? (parts + per - 1) / per : parts);
+        s.wg0 = (u32)wgs[1];
+        s.grp0 = (u32)(pl.floats / CK_WKEYS);
+        wgs[1] += (u64)s.ncb * n_kv * s.ns;
+        pl.floats += (u64)s.ncb * n_kv * s.ns * CK_WKEYS;
+    }
+    if (wgs[0] > 0x7fffffffull || wgs[1] > 0x7fffffffull) return false;
+    pl.wgs[0] = (u32)wgs[0];
+    pl.wgs[1] = (u32)wgs[1];
+    pl.blocks = (u32)blocks;
+    return true;
+}
+
+static bool most_sums(u32 n_kv, u32 gqa, u32 window, const tl_chunk *ch, u32 n_chunk, u64 *floats) {
+    WeightPlan pl;
+    const tl_chunk *of[CK_MAX_SEQ];
+    *floats = 0;
+    for (u32 i = 0; i < n_chunk;) {
+        const u32 m = next_chunks(ch, n_chunk, &i, of);
+        if (!m) break;
+        if (!plan_weight(pl, of, m, n_kv, gqa, window)) return false;
+        *floats = pl.floats > *floats ? pl.floats : *floats;
+    }
+    return true;
+}
+
 extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl_chunk_attn_args *a,
                                  const tl_chunk *chunks, uint32_t n_chunk, uint64_t *bytes) {
     if (!a || !bytes || (n_chunk && !chunks) || n_chunk > CK_MAX_CHUNKS || !n_kv_head || !a->n_head ||
         a->n_head % n_kv_head || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return tl_fail(TL_EINVAL, "attn_chunks_ws: arguments");
-    u64 parts;
-    if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, a->window, chunks, n_chunk, &parts))
+    u64 parts, floats;
+    if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, a->window, chunks, n_chunk, &parts) ||
+        !most_sums(n_kv_head, a->n_head / n_kv_head, a->window, chunks, n_chunk, &floats))
         return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
-    *bytes = ws_need(parts, head_dim);
+    const u64 attn = ws_need(parts, head_dim), weight = CK_WS_HEAD + floats * sizeof(float);
+    *bytes = attn > weight ? attn : weight;
     return TL_OK;
 }
 
-/* where the call's counters, pairs and partial rows lie (its launches take
- * them one after another) */
-static int take_ws(const tl_chunk_attn_args *a, u64 parts, u32 head_dim, hipStream_t st, CkAttnParams &p) {
-    if (!parts) return TL_OK;
+/* where the call's counters, (max, sum) pairs and partial floats lie (its
+ * launches take them one after another) */
+static int take_ws(const tl_chunk_attn_args *a, u64 pairs, u64 floats, hipStream_t st, CkAttnParams &p) {
+    if (!floats) return TL_OK;
     if (a->ws) {
-        const u64 need = ws_need(parts, head_dim);
+        const u64 need = CK_WS_HEAD + pairs * sizeof(float2) + floats * sizeof(float);
         if (a->ws_bytes < need)
             return tl_fail(TL_ERANGE, "attn_chunks: workspace of %llu bytes, %llu needed",
                            (unsigned long long)a->ws_bytes, (unsigned long long)need);
         p.cnt = (u32 *)a->ws;
         p.ws_ml = (float2 *)((char *)a->ws + CK_WS_HEAD);
-        p.ws_acc = (float *)(p.ws_ml + parts);
+        p.ws_acc = (float *)(p.ws_ml + pairs);
         return TL_OK;
     }
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
@@ -476,7 +544,7 @@ static int take_ws(const tl_chunk_attn_args *a, u64 parts, u32 head_dim, hipStre
     if (cs != hipStreamCaptureStatusNone)
         return tl_fail(TL_EINVAL, "attn_chunks: a captured call takes its own workspace (ws)");
     TlWorkspace *w;
-    const int rc = tl_workspace_get(st, parts * head_dim, parts, TL_MERGE_CNT_WORDS, &w);
+    const int rc = tl_workspace_get(st, floats, pairs, TL_MERGE_CNT_WORDS, &w);
     if (rc) return rc;
     p.cnt = w->cnt;
     p.ws_ml = (float2 *)w->ml;
@@ -513,7 +581,7 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
     u64 parts;
     if (!most_parts(L.n_kv_head, p.gqa, L.head_dim, a->window, ch, n_chunk, &parts))
         return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
-    rc = take_ws(a, parts, L.head_dim, st, p);
+    rc = take_ws(a, parts, parts * L.head_dim, st, p);
     if (rc) return rc;
     const tl_chunk *of[CK_MAX_SEQ];
     AttnPlan pl;
@@ -566,6 +634,26 @@ extern "C" int tl_attn_chunks_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_ar
 /* attention weight                                                          */
 /* ------------------------------------------------------------------------ */
 
+/* weight[key] += the sums of the kv heads and column shares, in order */
+__global__ __launch_bounds__(256) void chunk_weight_sum_kernel(const CkAttnParams p) {
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
+    const u32 kblk = blockIdx.x - sq.wg0;
+    const u32 key = sq.part0 + kblk * CK_WKEYS + threadIdx.x;
+    if (key >= sq.pos + sq.n) return;
+    const float *in = p.ws_acc + ((u64)sq.grp0 + kblk) * CK_WKEYS + threadIdx.x;
+    const u32 n = sq.ns * p.c.n_kv;
+    const float old = sq.weight[key];
+    float sum = 0.f;
+    for (u32 x = 0; x < n; x += 8) {
+        float v[8];
+#pragma unroll
+        for (u32 j = 0; j < 8; j++) v[j] = in[(u64)min(x + j, n - 1) * sq.ncb * CK_WKEYS];
+#pragma unroll
+        for (u32 j = 0; j < 8; j++) sum += x + j < n ? v[j] : 0.f;
+    }
+    sq.weight[key] = old + sum;
+}
+
 static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
                        hipStream_t st) {
     u32 shift;
@@ -580,22 +668,35 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
         return tl_fail(TL_EINVAL, "attn_weight: two chunks share weights");
     CkAttnParams p;
     fill_attn(p, L, a, shift);
+    u64 floats;
+    if (!most_sums(L.n_kv_head, p.gqa, a->window, ch, n_chunk, &floats))
+        return tl_fail(TL_ERANGE, "attn_weight: too many keys");
+    rc = take_ws(a, 0, floats, st, p);
+    if (rc) return rc;
     const tl_chunk *of[CK_MAX_SEQ];
+    WeightPlan pl;
     for (u32 i = 0; i < n_chunk;) {
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        p.n_seq = m;
-        u64 wgs = 0;
-        for (u32 j = 0; j < m; j++) {
-            seq_of(p.seq[j], *of[j]);
-            p.seq[j].wg0 = (u32)wgs;
-            p.seq[j].ncb = (u32)(((u64)p.seq[j].n * p.gqa + CK_COLS - 1) / CK_COLS);
-            wgs += ((u64)p.seq[j].pos + p.seq[j].n + CK_KEYS - 1) / CK_KEYS;
+        plan_weight(pl, of, m, L.n_kv_head, p.gqa, a->window);
+        for (int w = 1; w >= 0; w--) {
+            if (!pl.n[w]) continue;
+            p.n_seq = pl.n[w];
+            memcpy(p.seq, pl.seq[w], pl.n[w] * sizeof(CkSeq));
+            starts(p);
+            if (w) ck_launch_weight_wide(p, L.head_dim, L.q8, pl.wgs[w], st);
+            else ck_launch_weight(p, L.head_dim, L.q8, pl.wgs[w], st);
+            HIP_TRY(hipGetLastError());
+            if (!w) continue;
+            u32 at = 0;
+            for (u32 j = 0; j < pl.n[1]; j++) {
+                p.seq[j].wg0 = at;
+                at += p.seq[j].ncb;
+            }
+            starts(p);
+            hipLaunchKernelGGL(chunk_weight_sum_kernel, dim3(at), dim3(256), 0, st, p);
+            HIP_TRY(hipGetLastError());
         }
-        if (wgs > 0x7fffffffull) return tl_fail(TL_ERANGE, "attn_weight: too many keys");
-        starts(p);
-        ck_launch_weight(p, L.head_dim, L.q8, (u32)wgs, st);
-        HIP_TRY(hipGetLastError());
     }
     return TL_OK;
 }
@@ -626,6 +727,12 @@ void ck_launch_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipSt
     if (head_dim == 64) q8 ? ck_launch_wide_t<64, true>(p, wgs, st) : ck_launch_wide_t<64, false>(p, wgs, st);
     else if (head_dim == 128) q8 ? ck_launch_wide_t<128, true>(p, wgs, st) : ck_launch_wide_t<128, false>(p, wgs, st);
     else q8 ? ck_launch_wide_t<256, true>(p, wgs, st) : ck_launch_wide_t<256, false>(p, wgs, st);
+}
+
+void ck_launch_weight_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) q8 ? ck_launch_weight_wide_t<64, true>(p, wgs, st) : ck_launch_weight_wide_t<64, false>(p, wgs, st);
+    else if (head_dim == 128) q8 ? ck_launch_weight_wide_t<128, true>(p, wgs, st) : ck_launch_weight_wide_t<128, false>(p, wgs, st);
+    else q8 ? ck_launch_weight_wide_t<256, true>(p, wgs, st) : ck_launch_weight_wide_t<256, false>(p, wgs, st);
 }
 
 void ck_launch_weight(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {

@@ -24,14 +24,24 @@ void ck_launch_weight_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
     else
         hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, false>), dim3(wgs), dim3(256), 0, st, p);
 }
+template <int D, bool Q8>
+void ck_launch_weight_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
+    if (p.softcap > 0.f || p.slopes)
+        hipLaunchKernelGGL((chunk_weight_wide_kernel<D, Q8, true>), dim3(wgs), dim3(512), 0, st, p);
+    else
+        hipLaunchKernelGGL((chunk_weight_wide_kernel<D, Q8, false>), dim3(wgs), dim3(512), 0, st, p);
+}
 template void ck_launch_attn_t<64, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_attn_t<128, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_attn_t<256, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_weight_t<64, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_weight_t<128, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_weight_t<256, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_weight_wide_t<64, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_wide_t<64, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_weight_wide_t<128, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_wide_t<128, false>(const CkAttnParams &, u32, hipStream_t);
+template void ck_launch_weight_wide_t<256, false>(const CkAttnParams &, u32, hipStream_t);
 template void ck_launch_wide_t<256, false>(const CkAttnParams &, u32, hipStream_t);
 
 void ck_launch_merge(const CkAttnParams &p, u32 head_dim, u32 wgs, hipStream_t st) {

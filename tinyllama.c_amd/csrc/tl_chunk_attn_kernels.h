@@ -37,9 +37,11 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
     const u64 brow = (u64)sq.row + r;
 
     CkSees see;
-    see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
+    const u32 first = p.first ? p.first[brow] : 0;
+    see.set(pq, end, p.window, sq.prefix, first);
     CkSpan span;
-    span.set<16>(see);
+    span.set(sq.pos + c0 / p.gqa, sq.pos + (c0 + ncol - 1) / p.gqa, end, p.window, sq.prefix,
+             p.first ? ck_uniform(group_umin<16>(first)) : 0, p.first ? ck_uniform(group_umax<16>(first)) : 0);
     CkTiles<CK_KEYS> tiles;
     tiles.set(span);
     const u32 n_tiles = tiles.count();
@@ -65,7 +67,6 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
     if (t < t1) row = look(t);
     float4 qx[KS][2];
     ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, qx);
-    const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
     if (t < t1) {
         const u32 rc = row < p.c.cap ? row : 0;
         u32 rk[2], rv[8];
@@ -76,9 +77,9 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
         if (t + NW < t1) next = look(t + NW);
     }
     h8_t qh[KS], ql[KS];
-    float cs = ck_split_q<D, 4>(qx, p.scale, qh, ql);
-    if constexpr (!BIAS) cs *= CK_LOG2E;
-    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+    CkScore<BIAS> score;
+    score.set(p, ck_split_q<D, 4>(qx, p.scale, qh, ql), head);
+    const float mul = score.factor();
     float m = -INFINITY, l = 0.f;
     f4_t o[NM];
 #pragma unroll
@@ -100,9 +101,9 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
                 if constexpr (Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], acc, 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                x[4 * a + e] = ck_score<BIAS>(acc[e], cs, p.softcap, icap, slope, pq, kb + 8 * g + 4 * a + e);
+            for (int e = 0; e < 4; e++) x[4 * a + e] = acc[e];
         }
+        score.template apply<8>(x, (int)(pq - kb - 8 * g), [](int e) { return e; });
         u32 rn = 0;
         if (more) {
             rn = next < p.c.cap ? next : 0;
@@ -133,6 +134,7 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
         float top = x[0];
 #pragma unroll
         for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
+        top *= mul;
         const float thr = m == -INFINITY ? -INFINITY : m + CK_LAZY;
         if (__any(top > thr)) {
             top = fmaxf(top, __shfl_xor(top, 16));
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
         float l1 = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const float a = __builtin_amdgcn_exp2f(x[e] - mref), b = __builtin_amdgcn_exp2f(x[e + 1] - mref);
+            const float a = __builtin_amdgcn_exp2f(fmaf(x[e], mul, -mref)), b = __builtin_amdgcn_exp2f(fmaf(x[e + 1], mul, -mref));
             l += a;
             l1 += b;
             u32 hi, lo;
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     __shared__ __align__(16) u32 s_row[2][KT];   /* pool rows of a tile's keys, 0 for the bad ones */
     __shared__ u64 s_bad[4];                     /* keys of a tile without a row */
     __shared__ u64 s_odd[2][4];                  /* keys of a tile whose V is not all finite */
-    __shared__ CkSpan s_span[4];
+    __shared__ u32 s_first[2][4];
     const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
     const u32 i = lane & 31, h = lane >> 5;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
@@ -406,43 +408,41 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     const u32 end = sq.pos + sq.n;
     u32 pq;
     h8_t qh[NS], ql[NS];
-    float cs, slope = 0.f;
+    CkScore<BIAS> score;
     CkSees see;
+    CkSpan span;
     {
         const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
         const u64 brow = (u64)sq.row + r;
         pq = sq.pos + r;
-        see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
-        if (BIAS && p.slopes) slope = p.slopes[head];
+        const u32 first = p.first ? p.first[brow] : 0;
+        see.set(pq, end, p.window, sq.prefix, first);
+        span.set(sq.pos + min(cw, cols - 1) / p.gqa, sq.pos + min(cw + 31, cols - 1) / p.gqa, end, p.window, sq.prefix,
+                 p.first ? ck_uniform(group_umin<32>(first)) : 0, p.first ? ck_uniform(group_umax<32>(first)) : 0);
         float4 qx[NS][2];
         ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
-        cs = ck_split_q<D, 2>(qx, p.scale, qh, ql);
-        if constexpr (!BIAS) cs *= CK_LOG2E;
+        score.set(p, ck_split_q<D, 2>(qx, p.scale, qh, ql), head);
     }
-    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+    const float mul = score.factor();
 
-    CkSpan span, all;
-    span.set<32>(see);
-    if (lane == 0) s_span[wave] = span;
-    __syncthreads();
-    all = s_span[0];
+    u32 fmin = span.fmin, fmax = span.max_f;
+    if (p.first) {
+        if (lane == 0) {
+            s_first[0][wave] = fmin;
+            s_first[1][wave] = fmax;
+        }
+        __syncthreads();
 #pragma unroll
-    for (int w = 1; w < 4; w++) {
-        const CkSpan &o = s_span[w];
-        all.fmin = min(all.fmin, o.fmin);
-        all.lo = min(all.lo, o.lo);
-        all.hi = max(all.hi, o.hi);
-        all.max_lo = max(all.max_lo, o.max_lo);
-        all.min_hi = min(all.min_hi, o.min_hi);
-        all.max_f = max(all.max_f, o.max_f);
+        for (int w = 0; w < 4; w++) {
+            fmin = min(fmin, s_first[0][w]);
+            fmax = max(fmax, s_first[1][w]);
+        }
+        fmin = ck_uniform(fmin);
+        fmax = ck_uniform(fmax);
     }
-    all.fmin = ck_uniform(all.fmin);
-    all.lo = ck_uniform(all.lo);
-    all.hi = ck_uniform(all.hi);
-    all.max_lo = ck_uniform(all.max_lo);
-    all.min_hi = ck_uniform(all.min_hi);
-    all.max_f = ck_uniform(all.max_f);
-    all.pre = ck_uniform(all.pre);
+    CkSpan all;
+    all.set(sq.pos + cb * CK_WCOLS / p.gqa, sq.pos + min(cb * CK_WCOLS + CK_WCOLS - 1, cols - 1) / p.gqa, end, p.window,
+            sq.prefix, fmin, fmax);
     CkTiles<KT> tiles;
     tiles.set(all);
     const u32 n_tiles = tiles.count();
@@ -655,11 +655,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if constexpr (BIAS) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        s[e] = ck_score<true>(s[e], cs, p.softcap, icap, slope, pq, kb + 16 * (e >> 3) + 8 * h + (e & 7));
-                }
+                score.template apply<16>(s, (int)(pq - kb - 8 * h), [](int e) { return 16 * (e >> 3) + (e & 7); });
                 const u32 bad = (u32)(s_bad[(t - t0) & 3] >> (32 * sub));
                 if (!span.full(kb, 32) || bad) {
                     const u32 odd = (u32)((Q8 ? s_odd[buf][2] | s_odd[buf][3]
@@ -675,7 +671,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                 float top = s[0];
 #pragma unroll
                 for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-                if constexpr (!BIAS) top *= cs;
+                top *= mul;
                 const float thr = m == -INFINITY ? -INFINITY : m + CK_LAZY;
                 if (__any(top > thr)) {
                     top = fmaxf(top, __shfl_xor(top, 32));
@@ -700,8 +696,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                 float l1 = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                    const float a = __builtin_amdgcn_exp2f(BIAS ? s[e] - mref : fmaf(s[e], cs, -mref));
-                    const float b = __builtin_amdgcn_exp2f(BIAS ? s[e + 1] - mref : fmaf(s[e + 1], cs, -mref));
+                    const float a = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -mref));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(s[e + 1], mul, -mref));
                     l += a;
                     l1 += b;
                     u32 hi, lo;

@@ -13,3 +13,6 @@ template <int D, bool Q8>
 void ck_launch_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st);
 template <int D, bool Q8>
 void ck_launch_weight_t(const CkAttnParams &p, u32 wgs, hipStream_t st);
+void ck_launch_weight_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st);
+template <int D, bool Q8>
+void ck_launch_weight_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st);

@@ -4,7 +4,7 @@
 #pragma once
 #include "tl_chunk.h"
 
-/* One workgroup per tile of 32 keys of a chunk; its waves take the kv heads in
+/* Few columns: one workgroup per tile of 32 keys of a chunk; its waves take the kv heads in
  * turn, each with the tile's K as the matrix operand in registers against all
  * column blocks of the head.  A lane sums its eight keys over its columns; the
  * 16 lanes of a key and then the waves are joined in a fixed order. */
@@ -15,7 +15,7 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u32 i = lane & 15, g = lane >> 4;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
-    const u32 kb = (blockIdx.x - sq.wg0) * CK_KEYS;
+    const u32 kb = sq.part0 + (blockIdx.x - sq.wg0) * CK_KEYS;
     const u32 end = sq.pos + sq.n, cols = sq.n * p.gqa;
     const u32 key = kb + (lane & 31);
     const u32 row = key < end ? ck_row(p.c, sq.pages, key) : ~0u;
@@ -24,7 +24,6 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
     u32 rk[2];
 #pragma unroll
     for (int a = 0; a < 2; a++) rk[a] = __shfl(rc, 8 * (i >> 2) + 4 * a + (i & 3));
-    const float icap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
     float sum[8] = {};
     for (u32 kvh = wave; kvh < p.c.n_kv; kvh += 4) {
         CkTile<D, Q8> tile;
@@ -45,10 +44,11 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
             h8_t qh[KS], ql[KS];
             float4 qx[KS][2];
             ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, qx);
-            float cs = ck_split_q<D, 4>(qx, p.scale, qh, ql);
-            if constexpr (!BIAS) cs *= CK_LOG2E;
-            const float slope = BIAS && p.slopes ? p.slopes[head] : 0.f;
+            CkScore<BIAS> score;
+            score.set(p, ck_split_q<D, 4>(qx, p.scale, qh, ql), head);
+            const float mul = score.factor();
             const float lse = p.lse[brow * p.n_head + head] * CK_LOG2E;
+            float x[8];
 #pragma unroll
             for (int a = 0; a < 2; a++) {
                 f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -61,12 +61,13 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
                     if constexpr (Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], acc, 0, 0, 0);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const u32 k = kb + 8 * g + 4 * a + e;
-                    const float x = ck_score<BIAS>(acc[e], cs, p.softcap, icap, slope, pq, k);
-                    const bool vis = real && see.sees(k) && !((bad >> (8 * g + 4 * a + e)) & 1);
-                    sum[4 * a + e] += vis ? __builtin_amdgcn_exp2f(x - lse) : 0.f;
-                }
+                for (int e = 0; e < 4; e++) x[4 * a + e] = acc[e];
+            }
+            score.template apply<8>(x, (int)(pq - kb - 8 * g), [](int e) { return e; });
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const bool vis = real && see.sees(kb + 8 * g + e) && !((bad >> (8 * g + e)) & 1);
+                sum[e] += vis ? __builtin_amdgcn_exp2f(fmaf(x[e], mul, -lse)) : 0.f;
             }
         }
     }
@@ -79,5 +80,205 @@ __global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p)
     if (threadIdx.x < CK_KEYS && kb + threadIdx.x < end) {
         const u32 k = threadIdx.x;
         sq.weight[kb + k] += (s_sum[0][k] + s_sum[1][k]) + (s_sum[2][k] + s_sum[3][k]);
+    }
+}
+
+/* ---- many columns ------------------------------------------------------------
+ *
+ * A workgroup keeps 256 keys of one kv head in registers, 32 to a wave, as the A
+ * operand of v_mfma_f32_32x32x16_f16, and goes through a share of the head's
+ * columns: CT at a time are fetched, split into pairs of f16 and put to LDS by
+ * all 512 threads (two buffers, one barrier each), and every wave multiplies its
+ * keys with them.  A lane sums 16 keys over one column of 32; the lanes are
+ * joined at the end and the workgroup's sums go to its place in the workspace,
+ * which chunk_weight_sum_kernel adds up in order.  Bound by the matrix
+ * instructions (two products) and, with capped scores, by the vector ones. */
+typedef float f16w_t __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct CkWeight {
+    static constexpr int CT = D == 256 ? 32 : 64;     /* columns of a buffer */
+    static constexpr int TPC = 512 / CT;              /* threads of a column */
+    static constexpr int QV = D / 4 / TPC;            /* float4s of one of them */
+    static constexpr int U = D / 8;                   /* 16-byte units of a column's row */
+    static constexpr int PLANE = CT * U * 16;
+    static TL_DEV u32 at(u32 col, u32 unit) {
+        return (col * U + (unit ^ (U == 8 ? (col >> 1) & 7 : col & 15))) * 16;
+    }
+};
+
+template <int D, bool Q8, bool BIAS>
+__global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide_kernel(const CkAttnParams p) {
+    typedef CkWeight<D> W;
+    constexpr int NS = D / 16, CT = W::CT;
+    __shared__ __align__(16) char s_q[2][2][W::PLANE];    /* buffer, hi / lo */
+    __shared__ CkScore<BIAS> s_score[2][CT];
+    __shared__ CkSees s_see[2][CT];
+    __shared__ u32 s_pos[2][CT], s_first[2][CT];
+    __shared__ float s_lse[2][CT];
+    const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
+    const u32 i = lane & 31, h = lane >> 5;
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
+    /* ncb: key blocks from key part0 on; ns: shares of the columns; grp0: first set of sums */
+    const u32 local = blockIdx.x - sq.wg0;
+    const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
+    const u32 kblk = rest % sq.ncb, share = rest / sq.ncb;
+    const u32 end = sq.pos + sq.n, cols = sq.n * p.gqa;
+    const u32 kb = sq.part0 + kblk * CK_WKEYS + wave * 32;
+    const u32 tiles = (cols + CT - 1) / CT;
+    const u32 t0 = (u32)((u64)tiles * share / sq.ns), t1 = (u32)((u64)tiles * (share + 1) / sq.ns);
+
+    /* matrix row rho is key rho with bits 2 and 3 exchanged (any order would do) */
+    const u32 key = kb + ((i & 19) | ((i & 4) << 1) | ((i & 8) >> 1));
+    const u32 row = key < end ? ck_row(p.c, sq.pages, key) : ~0u;
+    const u32 rc = row < p.c.cap ? row : 0;
+    h8_t kh[NS], kl[Q8 ? NS : 1];
+    if constexpr (!Q8) {
+        const char *base = (const char *)(p.c.k + (u64)kvh * p.c.cap * D);
+#pragma unroll
+        for (int s = 0; s < NS; s++) kh[s] = *(const h8_t *)(base + (u64)(rc * (u32)(2 * D) + s * 32 + h * 16));
+    } else {
+        const char *base = (const char *)p.c.k + (u64)kvh * p.c.cap * D;
+        const u16 *sb = p.c.ks + (u64)kvh * p.c.cap * (D / 32);
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const uint2 v = *(const uint2 *)(base + (u64)(rc * (u32)D + s * 16 + h * 8));
+            const tl_half2 d2 = __builtin_bit_cast(tl_half2, (u32)sb[(u64)(rc * (u32)(D / 32) + (s >> 1))] * 0x10001u);
+            tl_half2 x[4];
+            i8x4_to_f16(v.x, x[0], x[1]);
+            i8x4_to_f16(v.y, x[2], x[3]);
+            u4_t a, b;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                u32 y, z;
+                ck_q8_pair(x[j], d2, y, z);
+                a[j] = y;
+                b[j] = z;
+            }
+            kh[s] = __builtin_bit_cast(h8_t, a);
+            kl[s] = __builtin_bit_cast(h8_t, b);
+        }
+    }
+
+    const u32 tc = threadIdx.x / W::TPC, tt = threadIdx.x % W::TPC;
+    float4 qx[W::QV];
+    auto fetch = [&](u32 t) {
+        const u32 c = min(t * CT + tc, cols - 1);
+        const u32 r = c / p.gqa, head = kvh * p.gqa + c % p.gqa;
+        const float *q = p.q + ((u64)sq.row + r) * p.q_stride + (u64)head * D + 4 * tt;
+#pragma unroll
+        for (int j = 0; j < W::QV; j++) qx[j] = *(const float4 *)(q + 4 * W::TPC * j);
+    };
+    auto store = [&](u32 t) {
+        const u32 buf = (t - t0) & 1, cg = t * CT + tc, c = min(cg, cols - 1);
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < W::QV; j++)
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(qx[j].x), fabsf(qx[j].y))), fmaxf(fabsf(qx[j].z), fabsf(qx[j].w)));
+        m = group_max<W::TPC>(m);
+        const int e = ck_row_exp(m);
+        const float up = __uint_as_float((u32)(e + 127) << 23);
+#pragma unroll
+        for (int j = 0; j < W::QV; j++) {
+            uint2 hi, lo;
+            ck_split2(qx[j].x * up, qx[j].y * up, hi.x, lo.x);
+            ck_split2(qx[j].z * up, qx[j].w * up, hi.y, lo.y);
+            const u32 f = W::TPC * j + tt;      /* float4 of the row */
+            const u32 at = W::at(tc, f >> 1) + (f & 1) * 8;
+            *(uint2 *)(s_q[buf][0] + at) = hi;
+            *(uint2 *)(s_q[buf][1] + at) = lo;
+        }
+        if (tt == 0) {
+            const u32 r = c / p.gqa, head = kvh * p.gqa + c % p.gqa, pq = sq.pos + r;
+            const u64 brow = (u64)sq.row + r;
+            const u32 first = p.first ? p.first[brow] : 0;
+            CkSees see;
+            see.set(pq, end, p.window, sq.prefix, first);
+            CkScore<BIAS> score;
+            score.set(p, __uint_as_float((u32)(127 - e) << 23) * p.scale, head);
+            s_see[buf][tc] = see;
+            s_score[buf][tc] = score;
+            s_pos[buf][tc] = pq;
+            s_first[buf][tc] = first;
+            /* columns past the last one count nothing */
+            s_lse[buf][tc] = cg < cols ? p.lse[brow * p.n_head + head] * CK_LOG2E : INFINITY;
+        }
+    };
+
+    float sum[16] = {};
+    if (t0 < t1) {
+        fetch(t0);
+        store(t0);
+    }
+#pragma unroll 1
+    for (u32 t = t0; t < t1; t++) {
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        const u32 buf = (t - t0) & 1;
+#pragma unroll 1
+        for (u32 sub = 0; sub < CT / 32; sub++) {
+            const u32 cb = t * CT + 32 * sub;
+            if (cb >= cols) break;
+            u32 fmin = 0, fmax = 0;
+            if (p.first) {
+                const u32 f = s_first[buf][32 * sub + i];
+                fmin = ck_uniform(group_umin<32>(f));
+                fmax = ck_uniform(group_umax<32>(f));
+            }
+            CkSpan span;
+            span.set(sq.pos + cb / p.gqa, sq.pos + min(cb + 31, cols - 1) / p.gqa, end, p.window, sq.prefix, fmin, fmax);
+            if (!span.any(kb, 32)) continue;
+            const u32 cl = 32 * sub + i;
+            u32 rd = W::at(cl, h);
+            asm volatile("" : "+v"(rd));
+            const char *qp = s_q[buf][0];
+            f16w_t s;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = 0.f;
+            constexpr int AHEAD = 4;
+            h8_t a[AHEAD], b[AHEAD];
+            auto read = [&](int j) {
+                const char *at = qp + (rd ^ (j * 32));
+                a[j % AHEAD] = *(const h8_t *)at;
+                b[j % AHEAD] = *(const h8_t *)(at + W::PLANE);
+            };
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) read(j);
+#pragma unroll
+            for (int j = 0; j < NS; j++) {
+                __builtin_amdgcn_sched_barrier(0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[j], a[j % AHEAD], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[j], b[j % AHEAD], s, 0, 0, 0);
+                if constexpr (Q8) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[j], a[j % AHEAD], s, 0, 0, 0);
+                if (j + AHEAD < NS) read(j + AHEAD);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const CkScore<BIAS> score = s_score[buf][cl];
+            const float mul = score.factor(), lse = s_lse[buf][cl];
+            score.template apply<16>(s, (int)(s_pos[buf][cl] - kb - 8 * h), [](int e) { return 16 * (e >> 3) + (e & 7); });
+            if (span.full(kb, 32)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e], mul, -lse));
+            } else {
+                const CkSees see = s_see[buf][cl];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const bool v = see.sees(kb + 16 * (e >> 3) + 8 * h + (e & 7));
+                    sum[e] += v ? __builtin_amdgcn_exp2f(fmaf(s[e], mul, -lse)) : 0.f;
+                }
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+    }
+    /* the columns' lanes joined; keys without a row count nothing */
+    const u64 bad = __ballot(row >= p.c.cap);
+    float *out = p.ws_acc + (u64)sq.grp0 * CK_WKEYS +
+                 ((u64)(share * p.c.n_kv + kvh) * sq.ncb + kblk) * CK_WKEYS + wave * 32;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const float x = group_sum<32>(sum[e]);
+        const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
+        const u32 rho = (k & 19) | ((k & 4) << 1) | ((k & 8) >> 1);      /* the lane that holds key k's row */
+        if (i == 0) out[k] = (bad >> rho) & 1 ? 0.f : x;
     }
 }
