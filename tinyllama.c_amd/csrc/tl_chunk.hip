@@ -345,7 +345,7 @@ struct AttnPlan {
 
 /* As many splits as fill the chip (narrow: one workgroup to a CU, wide: two, at
  * head_dim 256 one), none of fewer tiles than a narrow workgroup has waves, or
- * of fewer keys than 256 (wide: partial rows of 128 columns cost more to join). */
+ * of fewer keys than 128 (wide). */
 static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
                       u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
@@ -364,7 +364,7 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
     for (int w = 0; w < 2; w++) {
         const u32 fill = w && head_dim != 256 ? 512 : 256;
         u64 per = (total[w] + fill - 1) / fill, wgs = 0;
-        const u64 least = w || head_dim != 256 ? 8 : 4;
+        const u64 least = !w && head_dim != 256 ? 8 : 4;
         if (per < least) per = least;
         /* the smallest share whose workgroups all run at once, if there is one */
         u64 all = 0, most = 0;
@@ -457,7 +457,8 @@ struct WeightPlan {
  * through all heads of 32 keys, where reading K is the work. */
 #define CK_WEIGHT_WIDE_MIN 32
 
-static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 window) {
+static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
+                        bool q8, u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.blocks = 0;
     pl.floats = 0;
     u64 wgs[2] = {0, 0}, blocks = 0, shares = 0;
@@ -480,12 +481,24 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
             shares += (u64)s.ncb * ((cols + 127) / 128);
         }
     }
-    /* shares of 128 columns at least, two workgroups to a CU */
-    const u64 per = (shares * n_kv + 511) / 512;
+    /* shares of 128 columns at least, as many as run at once */
+    const u32 fill = head_dim == 64 && !q8 ? 512 : 256;
+    u64 per = (shares * n_kv + fill - 1) / fill;
+    if (per < 1) per = 1;
+    for (; blocks * n_kv <= fill; per++) {
+        u64 at_once = 0;
+        bool one = true;
+        for (u32 i = 0; i < pl.n[1]; i++) {
+            const u64 parts = ((u64)pl.seq[1][i].n * gqa + 127) / 128;
+            at_once += (u64)pl.seq[1][i].ncb * n_kv * ((parts + per - 1) / per);
+            one = one && parts <= per;
+        }
+        if (at_once <= fill || one) break;
+    }
     for (u32 i = 0; i < pl.n[1]; i++) {
         CkSeq &s = pl.seq[1][i];
         const u64 parts = ((u64)s.n * gqa + 127) / 128;
-        s.ns = (u32)(per > 1 ? (parts + per - 1) / per : parts);
+        s.ns = (u32)((parts + per - 1) / per);
         s.wg0 = (u32)wgs[1];
         s.grp0 = (u32)(pl.floats / CK_WKEYS);
         wgs[1] += (u64)s.ncb * n_kv * s.ns;
@@ -498,14 +511,15 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
     return true;
 }
 
-static bool most_sums(u32 n_kv, u32 gqa, u32 window, const tl_chunk *ch, u32 n_chunk, u64 *floats) {
+static bool most_sums(u32 n_kv, u32 gqa, u32 head_dim, bool q8, u32 window, const tl_chunk *ch, u32 n_chunk,
+                      u64 *floats) {
     WeightPlan pl;
     const tl_chunk *of[CK_MAX_SEQ];
     *floats = 0;
     for (u32 i = 0; i < n_chunk;) {
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        if (!plan_weight(pl, of, m, n_kv, gqa, window)) return false;
+        if (!plan_weight(pl, of, m, n_kv, gqa, head_dim, q8, window)) return false;
         *floats = pl.floats > *floats ? pl.floats : *floats;
     }
     return true;
@@ -516,11 +530,12 @@ extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl
     if (!a || !bytes || (n_chunk && !chunks) || n_chunk > CK_MAX_CHUNKS || !n_kv_head || !a->n_head ||
         a->n_head % n_kv_head || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return tl_fail(TL_EINVAL, "attn_chunks_ws: arguments");
-    u64 parts, floats;
+    u64 parts, floats[2];
     if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, a->window, chunks, n_chunk, &parts) ||
-        !most_sums(n_kv_head, a->n_head / n_kv_head, a->window, chunks, n_chunk, &floats))
+        !most_sums(n_kv_head, a->n_head / n_kv_head, head_dim, false, a->window, chunks, n_chunk, &floats[0]) ||
+        !most_sums(n_kv_head, a->n_head / n_kv_head, head_dim, true, a->window, chunks, n_chunk, &floats[1]))
         return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
-    const u64 attn = ws_need(parts, head_dim), weight = CK_WS_HEAD + floats * sizeof(float);
+    const u64 attn = ws_need(parts, head_dim), weight = CK_WS_HEAD + (floats[0] > floats[1] ? floats[0] : floats[1]) * sizeof(float);
     *bytes = attn > weight ? attn : weight;
     return TL_OK;
 }
@@ -669,7 +684,7 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
     CkAttnParams p;
     fill_attn(p, L, a, shift);
     u64 floats;
-    if (!most_sums(L.n_kv_head, p.gqa, a->window, ch, n_chunk, &floats))
+    if (!most_sums(L.n_kv_head, p.gqa, L.head_dim, L.q8, a->window, ch, n_chunk, &floats))
         return tl_fail(TL_ERANGE, "attn_weight: too many keys");
     rc = take_ws(a, 0, floats, st, p);
     if (rc) return rc;
@@ -678,7 +693,7 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
     for (u32 i = 0; i < n_chunk;) {
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        plan_weight(pl, of, m, L.n_kv_head, p.gqa, a->window);
+        plan_weight(pl, of, m, L.n_kv_head, p.gqa, L.head_dim, L.q8, a->window);
         for (int w = 1; w >= 0; w--) {
             if (!pl.n[w]) continue;
             p.n_seq = pl.n[w];

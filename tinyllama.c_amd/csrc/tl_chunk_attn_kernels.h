@@ -327,12 +327,14 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
 
 /* ---- many columns: 128 to a workgroup, K and V tiles shared through LDS ------
  *
- * Each of the four waves has 32 columns and runs S^T = K . Q^T and O^T += V^T .
- * P^T on v_mfma_f32_32x32x16_f16 (A rows: lane & 31, eight k's of half h = lane
- * >> 5).  A lane's sixteen scores of a 32-key block are rows (r & 3) + 8 (r >>
- * 2) + 4 h; matrix row rho is fed key rho with bits 2 and 3 exchanged, so they
- * are keys 16 u + 8 h + j (r = 8 u + j), the k order of step u of the second
- * product.
+ * A wave has 32 columns and runs S^T = K . Q^T and O^T += V^T . P^T on
+ * v_mfma_f32_32x32x16_f16 (A rows: lane & 31, eight k's of half h = lane >> 5).
+ * A lane's sixteen scores of a 32-key block are rows (r & 3) + 8 (r >> 2) + 4 h;
+ * matrix row rho is fed key rho with bits 2 and 3 exchanged, so they are keys 16
+ * u + 8 h + j (r = 8 u + j), the k order of step u of the second product.  At
+ * head_dim 256 q and O of 32 columns would take all registers of a SIMD (the
+ * compiler moved 370 accumulation registers per tile): there eight waves of 16
+ * columns on v_mfma_f32_16x16x32_f16, keys 8 h + e with h = lane >> 4.
  *
  * Tiles of KT keys, two buffers, one barrier each.  The pool rows of a tile are
  * looked up by one wave three tiles ahead and handed on through LDS; K rows go
@@ -343,17 +345,36 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
  * lanes' reads cover all banks.  A Q8_0 tile is kept as two planes, hi and lo,
  * both through registers (waves 0 and 1 K, waves 2 and 3 V). */
 typedef float f16_t __attribute__((ext_vector_type(16)));
+template <int MC>
+struct CkAcc {
+    typedef f16_t type;
+};
+template <>
+struct CkAcc<16> {
+    typedef f4_t type;
+};
+TL_DEV void ck_mfma(f16_t &c, h8_t a, h8_t b) { c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+TL_DEV void ck_mfma(f4_t &c, h8_t a, h8_t b) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+/* key of a lane's score e within 32 */
+template <int MC>
+TL_DEV constexpr int ck_key(int e) {
+    return MC == 32 ? 16 * (e >> 3) + (e & 7) : e;
+}
+
 
 template <int D, bool Q8>
 struct CkWide {
+    static constexpr int MC = D == 256 ? 16 : 32;    /* columns of a wave */
+    static constexpr int NW = CK_WCOLS / MC, NT = 64 * NW;
+    static constexpr int G = 64 / MC;                /* lanes of a column */
     static constexpr int KT = Q8 ? (D == 64 ? 64 : 32) : (D == 256 ? 32 : 64);
     static constexpr int U = D / 8;                  /* 16-byte units of a K row in LDS */
     static constexpr int VU = KT / 8;                /* ... of a V^T row */
     static constexpr int PL = Q8 ? 2 : 1;
-    static constexpr int VL = Q8 ? 128 : 256;        /* lanes that stage V */
+    static constexpr int VL = Q8 ? NT / 2 : NT;      /* lanes that stage V */
     static constexpr int DPL = KT * D / 8 / VL;      /* dims of V of one of them */
     static constexpr int RU = Q8 ? D / 16 : D / 8;   /* 16-byte units of a K row in memory */
-    static constexpr int KL = Q8 ? KT * RU / 128 : KT * D / 2048;   /* ... of a lane (Q8_0), of a wave / 64 */
+    static constexpr int KL = Q8 ? KT * RU / VL : KT * RU / NT;   /* ... of a staging lane */
     static constexpr int VD = Q8 ? DPL / 4 : DPL / 2;   /* dwords of V of a key and lane */
     static constexpr int ST = Q8 && KL * 4 > 8 * VD ? KL * 4 : 8 * VD;
     static constexpr int SC = Q8 ? 8 : 1;            /* scales of a staging lane */
@@ -361,7 +382,9 @@ struct CkWide {
     static constexpr int KP = KT * U * 16, VP = D * VU * 16;   /* bytes of a plane */
     /* byte offsets of units; exclusive-or linear in the bits of their arguments, so
      * an offset is the lane's part with a constant part put in (put) */
-    static constexpr TL_HOSTDEV u32 kswz(u32 key) { return U == 8 ? (key >> 1) & 7 : key & 15; }
+    static constexpr TL_HOSTDEV u32 kswz(u32 key) {
+        return U == 8 ? (key >> 1) & 7 : MC == 16 ? (key & 3) | ((key >> 1) & 12) : key & 15;
+    }
     static constexpr TL_HOSTDEV u32 kat(u32 key, u32 unit) { return (key * U + (unit ^ kswz(key))) * 16; }
     static constexpr TL_HOSTDEV u32 vat(u32 dim, u32 unit) {
         return (dim * VU + (unit ^ (VU == 8 ? ((dim >> 1) ^ (dim >> 3)) & 7 : (dim >> 2) & 3))) * 16;
@@ -386,45 +409,39 @@ TL_DEV void ck_lds_load16(void *to, const void *base, u32 off) {
 #define CK_AHEAD 4   /* LDS operand reads in flight ahead of the matrix instructions */
 
 template <int D, bool Q8, bool BIAS>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
+__global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
     typedef CkWide<D, Q8> W;
-    constexpr int KT = W::KT, NS = D / 16, NO = D / 32;
+    typedef typename CkAcc<W::MC>::type acc_t;
+    constexpr int KT = W::KT, MC = W::MC, G = W::G, NW = W::NW;
+    constexpr int SN = MC / 2;                       /* scores of a lane and 32 keys */
+    constexpr int NS = D / (8 * G);                  /* k-steps of the first product */
+    constexpr int NO = D / MC;                       /* blocks of O^T */
+    constexpr int VK = MC == 32 ? 2 : 1;             /* k-steps of the second product */
     /* buffer b, plane l of K: s_k + (b * PL + l) * KP; of V the same */
     __shared__ __align__(16) char s_k[2 * W::PL * W::KP];
     __shared__ __align__(16) char s_v[2 * W::PL * W::VP];
     __shared__ __align__(16) u32 s_row[2][KT];   /* pool rows of a tile's keys, 0 for the bad ones */
     __shared__ u64 s_bad[4];                     /* keys of a tile without a row */
-    __shared__ u64 s_odd[2][4];                  /* keys of a tile whose V is not all finite */
-    __shared__ u32 s_first[2][4];
+    __shared__ u64 s_odd[2][NW];                  /* keys of a tile whose V is not all finite */
+    __shared__ u32 s_first[2][NW];
     const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
-    const u32 i = lane & 31, h = lane >> 5;
+    const u32 i = lane & (MC - 1), h = lane / MC;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
-    const u32 cols = sq.n * p.gqa, cw = cb * CK_WCOLS + wave * 32;
+    const u32 cols = sq.n * p.gqa, cw = cb * CK_WCOLS + wave * MC;
     const bool live = cw < cols;
     const u32 col = min(cw + i, cols - 1);
     const u32 end = sq.pos + sq.n;
-    u32 pq;
-    h8_t qh[NS], ql[NS];
-    CkScore<BIAS> score;
+    const u32 pq = sq.pos + col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+    const u64 brow = (u64)sq.row + col / p.gqa;
     CkSees see;
     CkSpan span;
-    {
-        const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
-        const u64 brow = (u64)sq.row + r;
-        pq = sq.pos + r;
-        const u32 first = p.first ? p.first[brow] : 0;
-        see.set(pq, end, p.window, sq.prefix, first);
-        span.set(sq.pos + min(cw, cols - 1) / p.gqa, sq.pos + min(cw + 31, cols - 1) / p.gqa, end, p.window, sq.prefix,
-                 p.first ? ck_uniform(group_umin<32>(first)) : 0, p.first ? ck_uniform(group_umax<32>(first)) : 0);
-        float4 qx[NS][2];
-        ck_load_q<D, 2>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
-        score.set(p, ck_split_q<D, 2>(qx, p.scale, qh, ql), head);
-    }
-    const float mul = score.factor();
-
+    const u32 first = p.first ? p.first[brow] : 0;
+    see.set(pq, end, p.window, sq.prefix, first);
+    span.set(sq.pos + min(cw, cols - 1) / p.gqa, sq.pos + min(cw + MC - 1, cols - 1) / p.gqa, end, p.window, sq.prefix,
+             p.first ? ck_uniform(group_umin<MC>(first)) : 0, p.first ? ck_uniform(group_umax<MC>(first)) : 0);
     u32 fmin = span.fmin, fmax = span.max_f;
     if (p.first) {
         if (lane == 0) {
@@ -433,7 +450,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
         }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             fmin = min(fmin, s_first[0][w]);
             fmax = max(fmax, s_first[1][w]);
         }
@@ -447,13 +464,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     tiles.set(all);
     const u32 n_tiles = tiles.count();
     const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
-
-    float m = -INFINITY, l = 0.f;
-    f16_t o[NO];
-#pragma unroll
-    for (int b = 0; b < NO; b++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[b][e] = 0.f;
 
     /* staging */
     u32 st[W::ST];
@@ -474,7 +484,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
     };
     /* the places of a staging lane, kept out of registers across the tile loop */
     auto place = [&](u32 &sl) {
-        sl = Q8 ? (wave & 1) * 64 + lane : threadIdx.x;
+        sl = Q8 ? threadIdx.x % W::VL : threadIdx.x;
         asm volatile("" : "+v"(sl));
     };
     auto fetch = [&](u32 t) {
@@ -487,13 +497,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
             const u32 ln = sl & 63;
 #pragma unroll
             for (int j = 0; j < W::KL; j++) {
-                const u32 c = wave * W::KL + j, key = c * (64 / W::U) + ln / W::U;
+                const u32 c = wave * W::KL + j, key = (c * 64 + ln) / W::U;
                 ck_lds_load16(to + c * 1024, kbase, rows[key] * (u32)(2 * D) + ((ln % W::U) ^ W::kswz(key)) * 16);
             }
-        } else if (wave < 2) {
+        } else if (wave < NW / 2) {
 #pragma unroll
             for (int j = 0; j < W::KL; j++) {
-                const u32 u = sl % W::RU, row = rows[j * (128 / W::RU) + sl / W::RU];
+                const u32 u = sl % W::RU, row = rows[j * (W::VL / W::RU) + sl / W::RU];
                 const u4_t v = *(const u4_t *)(kbase + (u64)(row * (u32)(W::RU * 16) + u * 16));
 #pragma unroll
                 for (int d = 0; d < 4; d++) st[4 * j + d] = v[d];
@@ -522,12 +532,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
         place(sl);
         const u32 dg = sl % (D / W::DPL), kg = sl / (D / W::DPL);
         if constexpr (Q8)
-            if (wave < 2) {
+            if (wave < NW / 2) {
                 const u32 kst = W::kat(sl / W::RU, 2 * (sl % W::RU));
                 char *to = s_k + buf * (W::PL * W::KP);
 #pragma unroll
                 for (int j = 0; j < W::KL; j++) {
-                    const u32 c = W::kat(j * (128 / W::RU), 0);
+                    const u32 c = W::kat(j * (W::VL / W::RU), 0);
                     const tl_half2 d2 = __builtin_bit_cast(tl_half2, sc[j] * 0x10001u);
                     u32 hi[8], lo[8];
 #pragma unroll
@@ -602,18 +612,33 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
         }
     };
 
-    u32 next = 0;
+    /* the first tiles' rows, q and the first tile are requested one after another
+     * and waited for together */
+    u32 next = 0, ra = 0, rb = 0;
+    if (wave == 0 && t0 < t1) {
+        ra = look(t0);
+        if (t0 + 1 < t1) rb = look(t0 + 1);
+        if (t0 + 2 < t1) next = look(t0 + 2);
+    }
+    float4 qx[NS][2];
+    ck_load_q<D, G>(p.q + brow * p.q_stride + (u64)head * D, h, qx);
     if (t0 < t1) {
         if (wave == 0) {
-            const u32 a = look(t0), b = t0 + 1 < t1 ? look(t0 + 1) : 0;
-            if (t0 + 2 < t1) next = look(t0 + 2);
-            hand_on(t0, a);
-            if (t0 + 1 < t1) hand_on(t0 + 1, b);
+            hand_on(t0, ra);
+            if (t0 + 1 < t1) hand_on(t0 + 1, rb);
         }
         __syncthreads();
         fetch(t0);
-        store(t0);
     }
+    h8_t qh[NS], ql[NS];
+    CkScore<BIAS> score;
+    score.set(p, ck_split_q<D, G>(qx, p.scale, qh, ql), head);
+    const float mul = score.factor();
+    float m = -INFINITY, l = 0.f;
+    acc_t o[NO];
+#pragma unroll
+    for (int b = 0; b < NO; b++) o[b] = (acc_t)(0.f);
+    if (t0 < t1) store(t0);
 #pragma unroll 1
     for (u32 t = t0; t < t1; t++) {
         const u32 kt = tiles.key(t);
@@ -629,40 +654,49 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
             u32 ii = i;
             asm volatile("" : "+v"(ii));
             const char *const kp = s_k + buf * (W::PL * W::KP), *const vp = s_v + buf * (W::PL * W::VP);
-            const u32 krd = W::kat((ii & 19) | ((ii & 4) << 1) | ((ii & 8) >> 1), h), vrd = W::vat(ii, h);
+            const u32 krd = W::kat(MC == 32 ? (ii & 19) | ((ii & 4) << 1) | ((ii & 8) >> 1) : (ii & 3) | ((ii & 12) << 1), h);
+            const u32 vrd = W::vat(ii, h);
 #pragma unroll
             for (int sub = 0; sub < KT / 32; sub++) {
                 const u32 kb = kt + 32 * sub;
-                f16_t s;
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = 0.f;
+                float s[SN];
                 {
+                    /* MC = 16: two blocks of 16 keys, one after the other */
+                    constexpr int NR = MC == 32 ? NS : 2 * NS;
+                    acc_t acc[MC == 32 ? 1 : 2];
                     h8_t a[CK_AHEAD], b[CK_AHEAD];
                     auto read = [&](int j) {
-                        const char *at = kp + W::kput(krd, W::kat(32 * sub, 2 * j));
+                        const char *at = kp + W::kput(krd, MC == 32 ? W::kat(32 * sub, 2 * j) : W::kat(32 * sub + 4 * (j & 1), 4 * (j >> 1)));
                         a[j % CK_AHEAD] = *(const h8_t *)at;
                         if constexpr (Q8) b[j % CK_AHEAD] = *(const h8_t *)(at + W::KP);
                     };
+                    acc[0] = (acc_t)(0.f);
+                    if constexpr (MC == 16) acc[1] = (acc_t)(0.f);
 #pragma unroll
                     for (int j = 0; j < CK_AHEAD; j++) read(j);
 #pragma unroll
-                    for (int j = 0; j < NS; j++) {
+                    for (int j = 0; j < NR; j++) {
+                        const int k = MC == 32 ? j : j >> 1, c = MC == 32 ? 0 : j & 1;
                         __builtin_amdgcn_sched_barrier(0);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % CK_AHEAD], qh[j], s, 0, 0, 0);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[j % CK_AHEAD], ql[j], s, 0, 0, 0);
-                        if constexpr (Q8) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[j % CK_AHEAD], qh[j], s, 0, 0, 0);
-                        if (j + CK_AHEAD < NS) read(j + CK_AHEAD);
+                        ck_mfma(acc[c], a[j % CK_AHEAD], qh[k]);
+                        ck_mfma(acc[c], a[j % CK_AHEAD], ql[k]);
+                        if constexpr (Q8) ck_mfma(acc[c], b[j % CK_AHEAD], qh[k]);
+                        if (j + CK_AHEAD < NR) read(j + CK_AHEAD);
                     }
                     __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < SN; e++) s[e] = MC == 32 ? acc[0][e % (MC == 32 ? 16 : 4)] : acc[(e >> 2) & 1 & (MC == 32 ? 0 : 1)][e & 3];
                 }
-                score.template apply<16>(s, (int)(pq - kb - 8 * h), [](int e) { return 16 * (e >> 3) + (e & 7); });
+                score.template apply<SN>(s, (int)(pq - kb - 8 * h), [](int e) { return ck_key<MC>(e); });
                 const u32 bad = (u32)(s_bad[(t - t0) & 3] >> (32 * sub));
                 if (!span.full(kb, 32) || bad) {
-                    const u32 odd = (u32)((Q8 ? s_odd[buf][2] | s_odd[buf][3]
-                                              : s_odd[buf][0] | s_odd[buf][1] | s_odd[buf][2] | s_odd[buf][3]) >> (32 * sub));
+                    u64 keys = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
+                    for (int w = Q8 ? NW / 2 : 0; w < NW; w++) keys |= s_odd[buf][w];
+                    const u32 odd = (u32)(keys >> (32 * sub));
+#pragma unroll
+                    for (int e = 0; e < SN; e++) {
+                        const u32 k = ck_key<MC>(e) + 8 * h;
                         const bool v = see.sees(kb + k) && !((bad >> k) & 1);
                         s[e] = v ? s[e] : -INFINITY;
                         if (v && ((odd >> k) & 1)) l = NAN;
@@ -670,10 +704,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                 }
                 float top = s[0];
 #pragma unroll
-                for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+                for (int e = 1; e < SN; e++) top = fmaxf(top, s[e]);
                 top *= mul;
                 const float thr = m == -INFINITY ? -INFINITY : m + CK_LAZY;
                 if (__any(top > thr)) {
+                    if constexpr (MC == 16) top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const float mn = top > thr ? top : m;
                     const float al = m == -INFINITY ? (mn == m ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - mn);
@@ -685,17 +720,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                 const float mref = m == -INFINITY ? 0.f : m - CK_UP;
                 h8_t v[CK_AHEAD], w[CK_AHEAD];
                 auto read = [&](int j) {
-                    const char *at = vp + W::vput(vrd, W::vat(32 * (j % NO), 4 * sub + 2 * (j / NO)));
+                    const char *at = vp + W::vput(vrd, W::vat(MC * (j % NO), 4 * sub + 2 * (j / NO)));
                     v[j % CK_AHEAD] = *(const h8_t *)at;
                     if constexpr (Q8) w[j % CK_AHEAD] = *(const h8_t *)(at + W::VP);
                 };
 #pragma unroll
-                for (int j = 0; j < CK_AHEAD && j < 2 * NO; j++) read(j);
+                for (int j = 0; j < CK_AHEAD; j++) read(j);
                 __builtin_amdgcn_sched_barrier(0);
-                u4_t ph[2], pl[2];
+                u4_t ph[VK], pl[VK];
                 float l1 = 0.f;
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
+                for (int e = 0; e < SN; e += 2) {
                     const float a = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -mref));
                     const float b = __builtin_amdgcn_exp2f(fmaf(s[e + 1], mul, -mref));
                     l += a;
@@ -707,45 +742,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void chunk_attn_wide_kernel(
                 }
                 l += l1;
 #pragma unroll
-                for (int j = 0; j < 2 * NO; j++) {
+                for (int j = 0; j < VK * NO; j++) {
                     __builtin_amdgcn_sched_barrier(0);
                     const int b = j % NO, u = j / NO;
                     const h8_t x = __builtin_bit_cast(h8_t, ph[u]), y = __builtin_bit_cast(h8_t, pl[u]);
-                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % CK_AHEAD], x, o[b], 0, 0, 0);
-                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % CK_AHEAD], y, o[b], 0, 0, 0);
-                    if constexpr (Q8) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[j % CK_AHEAD], x, o[b], 0, 0, 0);
-                    if (j + CK_AHEAD < 2 * NO) read(j + CK_AHEAD);
+                    ck_mfma(o[b], v[j % CK_AHEAD], x);
+                    ck_mfma(o[b], v[j % CK_AHEAD], y);
+                    if constexpr (Q8) ck_mfma(o[b], w[j % CK_AHEAD], x);
+                    if (j + CK_AHEAD < VK * NO) read(j + CK_AHEAD);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (t + 1 < t1) store(t + 1);
     }
+    if constexpr (MC == 16) l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (!live || cw + i >= cols) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    /* block b, registers 4 e ..: dims MC b + 8 e + 4 h (MC = 16: 4 h) */
     if (sq.ns == 1) {
-        const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
-        const u64 brow = (u64)sq.row + r;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         float *d = p.dst + brow * p.q_stride + (u64)head * D + 4 * h;
 #pragma unroll
         for (int b = 0; b < NO; b++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                *(float4 *)(d + 32 * b + 8 * e) = make_float4(o[b][4 * e] * inv, o[b][4 * e + 1] * inv,
+            for (int e = 0; e < MC / 8 * MC / 32; e++)
+                *(float4 *)(d + MC * b + 8 * e) = make_float4(o[b][4 * e] * inv, o[b][4 * e + 1] * inv,
                                                              o[b][4 * e + 2] * inv, o[b][4 * e + 3] * inv);
         if (p.lse && h == 0)
             p.lse[brow * p.n_head + head] = l == 0.f ? -INFINITY
                 : ((m == -INFINITY ? 0.f : m) - CK_UP + __builtin_amdgcn_logf(l)) * CK_LN2;
         return;
     }
-    const u64 part = (u64)sq.part0 + ((u64)(kvh * sq.ncb + cb) * sq.ns + split) * CK_WCOLS + wave * 32 + i;
+    const u64 part = (u64)sq.part0 + ((u64)(kvh * sq.ncb + cb) * sq.ns + split) * CK_WCOLS + wave * MC + i;
     float *d = p.ws_acc + part * D + 4 * h;
 #pragma unroll
     for (int b = 0; b < NO; b++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            *(float4 *)(d + 32 * b + 8 * e) = make_float4(o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]);
+        for (int e = 0; e < MC / 8 * MC / 32; e++)
+            *(float4 *)(d + MC * b + 8 * e) = make_float4(o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]);
     if (h == 0) p.ws_ml[part] = make_float2(m, l);
 }
 
