@@ -454,14 +454,14 @@ struct WeightPlan {
 };
 
 /* More columns than this keep 256 keys of one head to a workgroup; fewer go
- * through all heads of 32 keys, where reading K is the work. */
-#define CK_WEIGHT_WIDE_MIN 32
+ * through all heads of a run of keys, where reading K is the work. */
+#define CK_WEIGHT_WIDE_MIN CK_COLS
 
 static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
                         bool q8, u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.blocks = 0;
     pl.floats = 0;
-    u64 wgs[2] = {0, 0}, blocks = 0, shares = 0;
+    u64 wgs[2] = {0, 0}, blocks = 0, shares = 0, tiles = 0;
     for (u32 i = 0; i < n; i++) {
         const u64 cols = (u64)ch[i]->n * gqa, end = (u64)ch[i]->pos + ch[i]->n;
         const int w = cols > CK_WEIGHT_WIDE_MIN;
@@ -470,16 +470,30 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
         /* first key that a window leaves (documents' starts are known on the device only) */
         u64 lo = window && (u64)ch[i]->pos + 1 > window && !ch[i]->prefix ? (u64)ch[i]->pos + 1 - window : 0;
         if (!w) {
-            s.ncb = (u32)((cols + CK_COLS - 1) / CK_COLS);
             s.part0 = (u32)(lo / CK_KEYS * CK_KEYS);
-            s.wg0 = (u32)wgs[0];
-            wgs[0] += (end - s.part0 + CK_KEYS - 1) / CK_KEYS;
+            tiles += (end - s.part0 + CK_KEYS - 1) / CK_KEYS;
         } else {
             s.part0 = (u32)(lo / CK_WKEYS * CK_WKEYS);
             s.ncb = (u32)((end - s.part0 + CK_WKEYS - 1) / CK_WKEYS);
             blocks += s.ncb;
             shares += (u64)s.ncb * ((cols + 127) / 128);
         }
+    }
+    /* few columns: the smallest run of tiles whose workgroups all run at once */
+    u64 run = (tiles + 255) / 256;
+    for (; pl.n[0]; run += 1 + run / 32) {
+        u64 at_once = 0;
+        for (u32 i = 0; i < pl.n[0]; i++) {
+            const CkSeq &s = pl.seq[0][i];
+            at_once += ((u64)s.pos + s.n - s.part0 + run * CK_KEYS - 1) / (run * CK_KEYS);
+        }
+        if (at_once <= 256 || run >= tiles) break;
+    }
+    for (u32 i = 0; i < pl.n[0]; i++) {
+        CkSeq &s = pl.seq[0][i];
+        s.ncb = (u32)run;
+        s.wg0 = (u32)wgs[0];
+        wgs[0] += ((u64)s.pos + s.n - s.part0 + run * CK_KEYS - 1) / (run * CK_KEYS);
     }
     /* shares of 128 columns at least, as many as run at once */
     const u32 fill = head_dim == 64 && !q8 ? 512 : 256;

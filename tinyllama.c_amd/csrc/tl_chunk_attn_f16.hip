@@ -20,9 +20,9 @@ void ck_launch_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
 template <int D, bool Q8>
 void ck_launch_weight_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {
     if (p.softcap > 0.f || p.slopes)
-        hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, true>), dim3(wgs), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, true>), dim3(wgs), dim3(512), 0, st, p);
     else
-        hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, false>), dim3(wgs), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((chunk_weight_kernel<D, Q8, false>), dim3(wgs), dim3(512), 0, st, p);
 }
 template <int D, bool Q8>
 void ck_launch_weight_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st) {

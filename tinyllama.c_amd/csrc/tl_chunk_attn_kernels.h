@@ -497,7 +497,7 @@ __global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel
             const u32 ln = sl & 63;
 #pragma unroll
             for (int j = 0; j < W::KL; j++) {
-                const u32 c = wave * W::KL + j, key = (c * 64 + ln) / W::U;
+                const u32 c = wave * W::KL + j, key = c * (64 / W::U) + ln / W::U;
                 ck_lds_load16(to + c * 1024, kbase, rows[key] * (u32)(2 * D) + ((ln % W::U) ^ W::kswz(key)) * 16);
             }
         } else if (wave < NW / 2) {

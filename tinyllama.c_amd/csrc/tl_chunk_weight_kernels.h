@@ -4,82 +4,123 @@
 #pragma once
 #include "tl_chunk.h"
 
-/* Few columns: one workgroup per tile of 32 keys of a chunk; its waves take the kv heads in
- * turn, each with the tile's K as the matrix operand in registers against all
- * column blocks of the head.  A lane sums its eight keys over its columns; the
- * 16 lanes of a key and then the waves are joined in a fixed order. */
+/* ---- few columns (at most 16) --------------------------------------------------
+ *
+ * Bound by the read of K.  A workgroup has a run of 32-key tiles of a chunk; each
+ * of its eight waves has one kv head (with fewer heads several waves share one
+ * and take its tiles in turn; with more, the heads come in groups of eight) and
+ * keeps that head's q in registers while K comes straight into the matrix operand
+ * layout, one tile ahead.  A lane sums its eight keys' probabilities; the 16
+ * columns are joined by DPP, the waves through LDS in order. */
+#define CK_WTILES 32   /* tiles of a workgroup between two joins */
+
 template <int D, bool Q8, bool BIAS>
-__global__ __launch_bounds__(256) void chunk_weight_kernel(const CkAttnParams p) {
+__global__ __launch_bounds__(512, D == 64 ? 4 : 2) void chunk_weight_kernel(const CkAttnParams p) {
     constexpr int KS = D / 32;
-    __shared__ float s_sum[4][CK_KEYS];
-    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr bool TWO = D < 256 || Q8;      /* room for two tiles' K */
+    __shared__ float s_sum[8][CK_WTILES][CK_KEYS];
+    const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
     const u32 i = lane & 15, g = lane >> 4;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
-    const u32 kb = sq.part0 + (blockIdx.x - sq.wg0) * CK_KEYS;
+    /* ncb: tiles of a workgroup; part0: the chunk's first key */
     const u32 end = sq.pos + sq.n, cols = sq.n * p.gqa;
-    const u32 key = kb + (lane & 31);
-    const u32 row = key < end ? ck_row(p.c, sq.pages, key) : ~0u;
-    const u64 bad = __ballot(row >= p.c.cap);
-    const u32 rc = row < p.c.cap ? row : 0;
-    u32 rk[2];
+    const u32 k0 = sq.part0 + (blockIdx.x - sq.wg0) * sq.ncb * CK_KEYS;
+    const u32 tiles = min(sq.ncb, (end - k0 + CK_KEYS - 1) / CK_KEYS);
+    const u32 share = p.c.n_kv >= 8 ? 1 : 8 / p.c.n_kv;       /* waves of a head */
+    const u32 groups = (p.c.n_kv + 7) / 8;
+    const u32 turn = wave / (8 / share);
+    const bool real = i < cols;
+    const u32 col = real ? i : cols - 1;
+    const u32 pq = sq.pos + col / p.gqa;
+    const u64 brow = (u64)sq.row + col / p.gqa;
+    const u32 first = p.first ? p.first[brow] : 0;
+    CkSees see;
+    see.set(pq, end, p.window, sq.prefix, first);
+    CkSpan span;
+    span.set(sq.pos, sq.pos + (cols - 1) / p.gqa, end, p.window, sq.prefix,
+             p.first ? ck_uniform(group_umin<16>(first)) : 0, p.first ? ck_uniform(group_umax<16>(first)) : 0);
+    auto look = [&](u32 t) -> u32 {
+        const u32 key = k0 + t * CK_KEYS + (lane & 31);
+        return key < end ? ck_row(p.c, sq.pages, key) : ~0u;
+    };
+    for (u32 b0 = 0; b0 < tiles; b0 += CK_WTILES) {
+        const u32 b1 = min(b0 + CK_WTILES, tiles);
+        for (u32 x = lane; x < CK_WTILES * CK_KEYS; x += 64) s_sum[wave][0][x] = 0.f;
+        for (u32 hg = 0; hg < groups; hg++) {
+            const u32 kvh = p.c.n_kv >= 8 ? hg * 8 + wave : wave % (8 / share);
+            if (kvh >= p.c.n_kv || turn >= share) continue;
+            const u32 head = kvh * p.gqa + col % p.gqa;
+            CkTile<D, Q8> tile, ahead;
+            auto load = [&](CkTile<D, Q8> &to, u32 row) {
+                const u32 rc = row < p.c.cap ? row : 0;
+                u32 rk[2];
 #pragma unroll
-    for (int a = 0; a < 2; a++) rk[a] = __shfl(rc, 8 * (i >> 2) + 4 * a + (i & 3));
-    float sum[8] = {};
-    for (u32 kvh = wave; kvh < p.c.n_kv; kvh += 4) {
-        CkTile<D, Q8> tile;
-        tile.load_k(p.c, kvh, rk, g);
-        for (u32 cb = 0; cb < sq.ncb; cb++) {
-            const u32 c = cb * CK_COLS + i;
-            const bool real = c < cols;
-            const u32 col = real ? c : cols - 1;
-            const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
-            const u32 pq = sq.pos + r;
-            const u64 brow = (u64)sq.row + r;
-            CkSees see;
-            see.set(pq, end, p.window, sq.prefix, p.first ? p.first[brow] : 0);
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < 8; e++) any |= see.sees(kb + 8 * g + e);
-            if (!__any(any && real)) continue;
-            h8_t qh[KS], ql[KS];
+                for (int a = 0; a < 2; a++) rk[a] = __shfl(rc, 8 * (i >> 2) + 4 * a + (i & 3));
+                to.load_k(p.c, kvh, rk, g);
+            };
+            u32 t = b0 + turn;
+            u32 row = t < b1 ? look(t) : 0, next = t + share < b1 ? look(t + share) : 0;
             float4 qx[KS][2];
             ck_load_q<D, 4>(p.q + brow * p.q_stride + (u64)head * D, g, qx);
+            float lse = p.lse[brow * p.n_head + head] * CK_LOG2E;
+            if (t < b1) load(tile, row);
+            h8_t qh[KS], ql[KS];
             CkScore<BIAS> score;
             score.set(p, ck_split_q<D, 4>(qx, p.scale, qh, ql), head);
             const float mul = score.factor();
-            const float lse = p.lse[brow * p.n_head + head] * CK_LOG2E;
-            float x[8];
+            lse = real ? lse : INFINITY;       /* columns past the last one count nothing */
+            for (; t < b1; t += share) {
+                const u32 kb = k0 + t * CK_KEYS;
+                const u64 bad = __ballot(row >= p.c.cap);
+                const u32 coming = next;
+                if (TWO && t + share < b1) load(ahead, coming);
+                row = next;
+                if (TWO && t + 2 * share < b1) next = look(t + 2 * share);
+                const bool any = span.any(kb, CK_KEYS);
+                float x[8];
+                if (any) {
 #pragma unroll
-            for (int a = 0; a < 2; a++) {
-                f4_t acc = {0.f, 0.f, 0.f, 0.f};
+                    for (int a = 0; a < 2; a++) {
+                        f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    h8_t kh, kl;
-                    tile.get_k(a, s, kh, kl);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s], acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[s], acc, 0, 0, 0);
-                    if constexpr (Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], acc, 0, 0, 0);
+                        for (int s = 0; s < KS; s++) {
+                            h8_t kh, kl;
+                            tile.get_k(a, s, kh, kl);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s], acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[s], acc, 0, 0, 0);
+                            if constexpr (Q8) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s], acc, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[4 * a + e] = acc[e];
+                    }
                 }
+                if constexpr (!TWO) {
+                    if (t + share < b1) load(tile, coming);
+                    if (t + 2 * share < b1) next = look(t + 2 * share);
+                }
+                if (any) {
+                    score.template apply<8>(x, (int)(pq - kb - 8 * g), [](int e) { return e; });
+                    const bool full = span.full(kb, CK_KEYS) && !bad;
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * a + e] = acc[e];
-            }
-            score.template apply<8>(x, (int)(pq - kb - 8 * g), [](int e) { return e; });
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool vis = real && see.sees(kb + 8 * g + e) && !((bad >> (8 * g + e)) & 1);
-                sum[e] += vis ? __builtin_amdgcn_exp2f(fmaf(x[e], mul, -lse)) : 0.f;
+                    for (int e = 0; e < 8; e++) {
+                        float pe = __builtin_amdgcn_exp2f(fmaf(x[e], mul, -lse));
+                        if (!full) pe = see.sees(kb + 8 * g + e) && !((bad >> (8 * g + e)) & 1) ? pe : 0.f;
+                        pe = group_sum<16>(pe);
+                        if (i == 0) s_sum[wave][t - b0][8 * g + e] += pe;
+                    }
+                }
+                if constexpr (TWO) tile = ahead;
             }
         }
-    }
+        __syncthreads();
+        for (u32 x = threadIdx.x; x < (b1 - b0) * CK_KEYS; x += 512) {
+            const u32 key = k0 + b0 * CK_KEYS + x;
+            float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float s = group_sum<16>(sum[e]);
-        if (i == 0) s_sum[wave][8 * g + e] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x < CK_KEYS && kb + threadIdx.x < end) {
-        const u32 k = threadIdx.x;
-        sq.weight[kb + k] += (s_sum[0][k] + s_sum[1][k]) + (s_sum[2][k] + s_sum[3][k]);
+            for (int w = 0; w < 8; w++) sum += s_sum[w][0][x];
+            if (key < end) sq.weight[key] += sum;
+        }
+        __syncthreads();
     }
 }
 
