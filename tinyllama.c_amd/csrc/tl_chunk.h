@@ -26,6 +26,7 @@ struct CkSeq {
     float *weight;
     u32 pos, n, row, prefix, rope_skip;
     u32 wg0, ncb, ns, part0, grp0;   /* part0 counts columns */
+    u32 wide;                        /* in a launch of both kinds: 128 columns to a workgroup */
 };
 
 struct CkCache {
@@ -267,7 +268,10 @@ struct CkTileF16 {
             }
         }
     }
-    static constexpr bool LO = false;
+    TL_DEV void take_k(const CkTileF16 &o) {
+#pragma unroll
+        for (int x = 0; x < 2 * KS; x++) kr[x / KS][x % KS] = o.kr[x / KS][x % KS];
+    }
     TL_DEV void get_k(int a, int s, h8_t &hi, h8_t &) const { hi = __builtin_bit_cast(h8_t, kr[a][s]); }
     TL_DEV void get_v(int m, h8_t &hi, h8_t &) const {
         u4_t x;
@@ -338,7 +342,12 @@ struct CkTileQ8 {
             sv[e] = *(const u16 *)(sb + (u64)(rv[e] * (u32)(KS * 2) + i * NB / 32 * 2));
         }
     }
-    static constexpr bool LO = true;
+    TL_DEV void take_k(const CkTileQ8 &o) {
+#pragma unroll
+        for (int x = 0; x < 2 * KS; x++) kr[x / KS][x % KS] = o.kr[x / KS][x % KS];
+#pragma unroll
+        for (int x = 0; x < KS; x++) sk[x / (KS / 2)][x % (KS / 2)] = o.sk[x / (KS / 2)][x % (KS / 2)];
+    }
     TL_DEV void get_k(int a, int s, h8_t &hi, h8_t &lo) const {
         const u32 d = (sk[a][s >> 1] >> (16 * (s & 1))) & 0xffffu;
         const tl_half2 d2 = __builtin_bit_cast(tl_half2, d * 0x10001u);

@@ -344,8 +344,9 @@ struct AttnPlan {
 #define CK_WIDE_MIN 32
 
 /* As many splits as fill the chip (narrow: one workgroup to a CU, wide: two, at
- * head_dim 256 one), none of fewer tiles than a narrow workgroup has waves, or
- * of fewer keys than 128 (wide). */
+ * head_dim 256 one; in one launch of both, up to head_dim 128, the narrow ones
+ * are of half the size and take what the wide ones leave), none of fewer tiles
+ * than a narrow workgroup has waves, or of fewer keys than 128 (wide). */
 static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
                       u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
@@ -361,10 +362,12 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
         tiles[w][pl.n[w]++] = span_tiles(*ch[i], window, 0, ch[i]->n);
         total[w] += tiles[w][pl.n[w] - 1] * s.ncb * n_kv;
     }
-    for (int w = 0; w < 2; w++) {
-        const u32 fill = w && head_dim != 256 ? 512 : 256;
+    const bool both = pl.n[0] && pl.n[1] && head_dim != 256;
+    for (int w = 1; w >= 0; w--) {
+        u32 fill = w && head_dim != 256 ? 512 : 256;
+        if (both && !w) fill = pl.wgs[1] < 384 ? 512 - pl.wgs[1] : 128;
         u64 per = (total[w] + fill - 1) / fill, wgs = 0;
-        const u64 least = !w && head_dim != 256 ? 8 : 4;
+        const u64 least = !w && head_dim != 256 && !both ? 8 : 4;
         if (per < least) per = least;
         /* the smallest share whose workgroups all run at once, if there is one */
         u64 all = 0, most = 0;
@@ -618,12 +621,22 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
         plan_attn(pl, of, m, L.n_kv_head, p.gqa, L.head_dim, a->window);
-        for (int w = 1; w >= 0; w--) {
+        const bool both = pl.n[0] && pl.n[1] && L.head_dim != 256;
+        for (int w = 1; w >= (both ? 1 : 0); w--) {
             if (!pl.wgs[w]) continue;
             p.n_seq = pl.n[w];
             memcpy(p.seq, pl.seq[w], pl.n[w] * sizeof(CkSeq));
+            if (both) {
+                /* the wide ones first: they take longer */
+                for (u32 j = 0; j < pl.n[1]; j++) p.seq[j].wide = 1;
+                for (u32 j = 0; j < pl.n[0]; j++) {
+                    p.seq[p.n_seq] = pl.seq[0][j];
+                    p.seq[p.n_seq++].wg0 += pl.wgs[1];
+                }
+            }
             starts(p);
-            if (w) ck_launch_wide(p, L.head_dim, L.q8, pl.wgs[w], st);
+            if (both) ck_launch_both(p, L.head_dim, L.q8, pl.wgs[0] + pl.wgs[1], st);
+            else if (w) ck_launch_wide(p, L.head_dim, L.q8, pl.wgs[w], st);
             else ck_launch_attn(p, L.head_dim, L.q8, pl.wgs[w], st);
             HIP_TRY(hipGetLastError());
             if (!w) continue;
@@ -756,6 +769,11 @@ void ck_launch_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipSt
     if (head_dim == 64) q8 ? ck_launch_wide_t<64, true>(p, wgs, st) : ck_launch_wide_t<64, false>(p, wgs, st);
     else if (head_dim == 128) q8 ? ck_launch_wide_t<128, true>(p, wgs, st) : ck_launch_wide_t<128, false>(p, wgs, st);
     else q8 ? ck_launch_wide_t<256, true>(p, wgs, st) : ck_launch_wide_t<256, false>(p, wgs, st);
+}
+
+void ck_launch_both(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {
+    if (head_dim == 64) q8 ? ck_launch_both_t<64, true>(p, wgs, st) : ck_launch_both_t<64, false>(p, wgs, st);
+    else q8 ? ck_launch_both_t<128, true>(p, wgs, st) : ck_launch_both_t<128, false>(p, wgs, st);
 }
 
 void ck_launch_weight_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st) {

@@ -15,16 +15,21 @@
 #define CK_LAZY 8.f
 #define CK_UP 7.f
 
-template <int D, bool Q8, bool BIAS>
-__global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const CkAttnParams p) {
-    constexpr int KS = D / 32, NM = D / 16, NW = CK_WAVES(D), NT = 64 * NW;
+template <int D, int NW>
+struct CkNarrowShared {
+    __align__(16) float o[NW * CK_COLS * (D + 4)];
+    float m[NW][CK_COLS], l[NW][CK_COLS];
+    u32 last;
+};
+
+template <int D, bool Q8, bool BIAS, int NW>
+TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, NW> &sh) {
+    constexpr int KS = D / 32, NM = D / 16, NT = 64 * NW;
     constexpr int ROWF = D + 4;
-    __shared__ __align__(16) float s_o[NW * CK_COLS * ROWF];
-    __shared__ float s_m[NW][CK_COLS], s_l[NW][CK_COLS];
-    __shared__ u32 s_last;
+    float *const s_o = sh.o;
+    float (&s_m)[NW][CK_COLS] = sh.m, (&s_l)[NW][CK_COLS] = sh.l;
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u32 i = lane & 15, g = lane >> 4;
-    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
@@ -47,7 +52,8 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
     const u32 n_tiles = tiles.count();
     const u32 t0 = (u32)((u64)n_tiles * split / sq.ns), t1 = (u32)((u64)n_tiles * (split + 1) / sq.ns);
 
-    CkTile<D, Q8> tile;
+    CkTile<D, Q8> tile, ahead;               /* of `ahead` only K: one tile further where registers allow */
+    constexpr bool TWO = D < 256;
     /* lane's key of a tile (the upper half of the wave repeats the lower) */
     auto look = [&](u32 t) -> u32 {
         const u32 key = tiles.key(t) + (lane & 31);
@@ -88,6 +94,13 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
         const u32 kb = tiles.key(t);
         const u64 bad = __ballot(row >= p.c.cap);
         const bool more = t + NW < t1;
+        u32 rn = 0;
+        if (TWO && more) {
+            rn = next < p.c.cap ? next : 0;
+            u32 rk[2];
+            rows_k(rn, rk);
+            ahead.load_k(p.c, kvh, rk, g);
+        }
         float x[8];
 #pragma unroll
         for (int a = 0; a < 2; a++) {
@@ -104,8 +117,7 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
             for (int e = 0; e < 4; e++) x[4 * a + e] = acc[e];
         }
         score.template apply<8>(x, (int)(pq - kb - 8 * g), [](int e) { return e; });
-        u32 rn = 0;
-        if (more) {
+        if (!TWO && more) {
             rn = next < p.c.cap ? next : 0;
             u32 rk[2];
             rows_k(rn, rk);
@@ -173,6 +185,7 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
             u32 rv[8];
             rows_v(rn, rv);
             tile.load_v(p.c, kvh, rv, i);
+            if constexpr (TWO) tile.take_k(ahead);
             row = next;
             if (t + 2 * NW < t1) next = look(t + 2 * NW);
         }
@@ -245,9 +258,9 @@ __global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const C
     __syncthreads();
     u32 *cnt = p.cnt + (u64)(sq.grp0 + group) * CK_CNT_PAD;
     if (threadIdx.x == 0)
-        s_last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sq.ns - 1;
+        sh.last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sq.ns - 1;
     __syncthreads();
-    if (!s_last) return;
+    if (!sh.last) return;
     u32 parts = 1;
     while (parts < NW && parts * 2 * units <= NT && parts * 8 < sq.ns) parts *= 2;
     const u32 run = (sq.ns + parts - 1) / parts;
@@ -408,8 +421,20 @@ TL_DEV void ck_lds_load16(void *to, const void *base, u32 off) {
 
 #define CK_AHEAD 4   /* LDS operand reads in flight ahead of the matrix instructions */
 
+template <int D, bool Q8>
+struct CkWideShared {
+    typedef CkWide<D, Q8> W;
+    /* buffer b, plane l of K: k + (b * PL + l) * KP; of V the same */
+    __align__(16) char k[2 * W::PL * W::KP];
+    __align__(16) char v[2 * W::PL * W::VP];
+    __align__(16) u32 row[2][W::KT];   /* pool rows of a tile's keys, 0 for the bad ones */
+    u64 bad[4];                        /* keys of a tile without a row */
+    u64 odd[2][W::NW];                 /* keys of a tile whose V is not all finite */
+    u32 first[2][W::NW];
+};
+
 template <int D, bool Q8, bool BIAS>
-__global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
+TL_DEV void ck_wide(const CkAttnParams &p, const CkSeq &sq, CkWideShared<D, Q8> &sh) {
     typedef CkWide<D, Q8> W;
     typedef typename CkAcc<W::MC>::type acc_t;
     constexpr int KT = W::KT, MC = W::MC, G = W::G, NW = W::NW;
@@ -417,16 +442,13 @@ __global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel
     constexpr int NS = D / (8 * G);                  /* k-steps of the first product */
     constexpr int NO = D / MC;                       /* blocks of O^T */
     constexpr int VK = MC == 32 ? 2 : 1;             /* k-steps of the second product */
-    /* buffer b, plane l of K: s_k + (b * PL + l) * KP; of V the same */
-    __shared__ __align__(16) char s_k[2 * W::PL * W::KP];
-    __shared__ __align__(16) char s_v[2 * W::PL * W::VP];
-    __shared__ __align__(16) u32 s_row[2][KT];   /* pool rows of a tile's keys, 0 for the bad ones */
-    __shared__ u64 s_bad[4];                     /* keys of a tile without a row */
-    __shared__ u64 s_odd[2][NW];                  /* keys of a tile whose V is not all finite */
-    __shared__ u32 s_first[2][NW];
+    char *const s_k = sh.k, *const s_v = sh.v;
+    u32 (&s_row)[2][KT] = sh.row;
+    u64 (&s_bad)[4] = sh.bad;
+    u64 (&s_odd)[2][NW] = sh.odd;
+    u32 (&s_first)[2][NW] = sh.first;
     const u32 lane = threadIdx.x & 63, wave = ck_uniform(threadIdx.x >> 6);
     const u32 i = lane & (MC - 1), h = lane / MC;
-    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
@@ -782,6 +804,34 @@ __global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel
         for (int e = 0; e < MC / 8 * MC / 32; e++)
             *(float4 *)(d + MC * b + 8 * e) = make_float4(o[b][4 * e], o[b][4 * e + 1], o[b][4 * e + 2], o[b][4 * e + 3]);
     if (h == 0) p.ws_ml[part] = make_float2(m, l);
+}
+
+template <int D, bool Q8, bool BIAS>
+__global__ __launch_bounds__(64 * CK_WAVES(D), 1) void chunk_attn_kernel(const CkAttnParams p) {
+    __shared__ CkNarrowShared<D, CK_WAVES(D)> sh;
+    ck_narrow<D, Q8, BIAS, CK_WAVES(D)>(p, p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)], sh);
+}
+
+template <int D, bool Q8, bool BIAS>
+__global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel(const CkAttnParams p) {
+    __shared__ CkWideShared<D, Q8> sh;
+    ck_wide<D, Q8, BIAS>(p, p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)], sh);
+}
+
+/* A batch of both kinds, head_dim 64 and 128: prompts' chunks and single tokens
+ * side by side in one launch, narrow workgroups of four waves.  (6 sessions of 1
+ * to 200 rows over a Q8_0 cache at 32/8/128: 39.7 us one after the other.) */
+template <int D, bool Q8, bool BIAS>
+__global__ __launch_bounds__(256, 2) void chunk_attn_both_kernel(const CkAttnParams p) {
+    static_assert(CkWide<D, Q8>::NT == 256, "one workgroup size");
+    __shared__ union {
+        char any[1];
+        CkWideShared<D, Q8> w;
+        CkNarrowShared<D, 4> n;
+    } sh;
+    const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
+    if (sq.wide) ck_wide<D, Q8, BIAS>(p, sq, sh.w);
+    else ck_narrow<D, Q8, BIAS, 4>(p, sq, sh.n);
 }
 
 /* The splits of the wide columns joined: D / 4 threads to a column, a float4

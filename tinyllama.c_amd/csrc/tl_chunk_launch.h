@@ -16,3 +16,6 @@ void ck_launch_weight_t(const CkAttnParams &p, u32 wgs, hipStream_t st);
 void ck_launch_weight_wide(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st);
 template <int D, bool Q8>
 void ck_launch_weight_wide_t(const CkAttnParams &p, u32 wgs, hipStream_t st);
+void ck_launch_both(const CkAttnParams &p, u32 head_dim, bool q8, u32 wgs, hipStream_t st);
+template <int D, bool Q8>
+void ck_launch_both_t(const CkAttnParams &p, u32 wgs, hipStream_t st);
