@@ -27,6 +27,7 @@ struct CkSeq {
     u32 pos, n, row, prefix, rope_skip;
     u32 wg0, ncb, ns, part0, grp0;   /* part0 counts columns */
     u32 wide;                        /* in a launch of both kinds: 128 columns to a workgroup */
+    u32 cb0;                         /* wide: its first column block (a band of the chunk's) */
 };
 
 struct CkCache {
@@ -44,7 +45,8 @@ struct CkAttnParams {
     const u32 *first;
     const float *slopes;
     u32 n_seq, n_head, gqa, q_stride, window;
-    float scale, softcap;
+    u32 gqa_mul;               /* x / gqa = high word of x * gqa_mul (gqa 1: 0) */
+    float scale, softcap, inv_cap;
     float *ws_acc;
     float2 *ws_ml;
     u32 *cnt;
@@ -66,6 +68,9 @@ typedef u32 u4_t __attribute__((ext_vector_type(4)));
 
 #define CK_LOG2E 1.4426950408889634f
 #define CK_LN2 0.6931471805599453f
+
+/* row and head of a column; exact below 2^32 / gqa, which the host sees to */
+TL_DEV u32 ck_row_of(const CkAttnParams &p, u32 col) { return p.gqa_mul ? __umulhi(col, p.gqa_mul) : col; }
 
 /* pool row of a session's position; ~0 where its page lies outside the pool */
 TL_DEV u32 ck_row(const CkCache &c, const u32 *pages, u32 p) {
@@ -441,7 +446,7 @@ TL_DEV float ck_split_q(const float4 (&x)[D / (8 * G)][2], float scale, h8_t (&h
 /* How products become scores in units of log2: s * mul after apply(). */
 template <bool BIAS>
 struct CkScore {
-    float mul, cap_in, slope, softcap;
+    float mul, cap_in, slope;
     bool capped, sloped;
     /* cs: factor from the products to scale * q.k */
     TL_DEV void set(const CkAttnParams &p, float cs, u32 head) {
@@ -450,13 +455,9 @@ struct CkScore {
             capped = p.softcap > 0.f;
             sloped = p.slopes != nullptr;
             slope = sloped ? p.slopes[head] * CK_LOG2E : 0.f;
-            softcap = p.softcap;
-            finish(cs);
+            if (capped) mul = p.softcap * CK_LOG2E;
+            cap_in = capped ? cs * p.inv_cap : 0.f;
         }
-    }
-    TL_DEV void finish(float cs) {
-        mul = capped ? softcap * CK_LOG2E : cs * CK_LOG2E;
-        cap_in = capped ? cs / softcap : 0.f;
     }
     /* far0: position minus the key of element 0; off(e): how far key e lies behind that */
     template <int N, class T, class F>

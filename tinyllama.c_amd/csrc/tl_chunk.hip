@@ -352,15 +352,27 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
     pl.parts = 0;
     u64 tiles[2][CK_MAX_SEQ], total[2] = {0, 0};
+    u32 n_wide = 0;
+    for (u32 i = 0; i < n; i++) n_wide += (u64)ch[i]->n * gqa > CK_WIDE_MIN;
     for (u32 i = 0; i < n; i++) {
         const u64 cols = (u64)ch[i]->n * gqa;
         const int w = cols > CK_WIDE_MIN;
-        CkSeq &s = pl.seq[w][pl.n[w]];
-        seq_of(s, *ch[i]);
         const u32 per = w ? CK_WCOLS : CK_COLS;
-        s.ncb = (u32)((cols + per - 1) / per);
-        tiles[w][pl.n[w]++] = span_tiles(*ch[i], window, 0, ch[i]->n);
-        total[w] += tiles[w][pl.n[w] - 1] * s.ncb * n_kv;
+        const u32 ncb = (u32)((cols + per - 1) / per);
+        /* bands of a wide chunk, each with splits by its own keys: its last rows see
+         * more than its first */
+        const u32 room = w ? 1 + (CK_MAX_SEQ - n) / n_wide : 1;
+        const u32 bands = room < ncb ? (room < 8 ? room : 8) : (ncb < 8 ? ncb : 8);
+        for (u32 b = 0; b < (w ? bands : 1); b++) {
+            CkSeq &s = pl.seq[w][pl.n[w]];
+            seq_of(s, *ch[i]);
+            const u32 b0 = w ? (u32)((u64)ncb * b / bands) : 0, b1 = w ? (u32)((u64)ncb * (b + 1) / bands) : ncb;
+            const u64 r1 = ((u64)b1 * per + gqa - 1) / gqa;
+            s.cb0 = b0;
+            s.ncb = b1 - b0;
+            tiles[w][pl.n[w]] = span_tiles(*ch[i], window, (u32)((u64)b0 * per / gqa), r1 < ch[i]->n ? (u32)r1 : ch[i]->n);
+            total[w] += tiles[w][pl.n[w]++] * s.ncb * n_kv;
+        }
     }
     const bool both = pl.n[0] && pl.n[1] && head_dim != 256;
     for (int w = 1; w >= 0; w--) {
@@ -421,6 +433,10 @@ static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_
         return tl_fail(TL_EINVAL, "attn_chunks: lse, first or slopes not aligned");
     if (!(a->scale > 0.f) || !isfinite(a->scale) || !(a->softcap >= 0.f) || !isfinite(a->softcap))
         return tl_fail(TL_EINVAL, "attn_chunks: scale %g softcap %g", (double)a->scale, (double)a->softcap);
+    const u64 gqa = a->n_head / L.n_kv_head;
+    for (u32 i = 0; i < n_chunk; i++)
+        if (ch[i].n * gqa > 0xffffffffull / gqa - CK_WCOLS)
+            return tl_fail(TL_ERANGE, "attn_chunks: %u rows of gqa %llu in a chunk", ch[i].n, (unsigned long long)gqa);
     if ((uintptr_t)a->ws & 15) return tl_fail(TL_EINVAL, "attn_chunks: workspace not 16-byte aligned");
     return TL_OK;
 }
@@ -598,6 +614,8 @@ static void fill_attn(CkAttnParams &p, const LayerView &L, const tl_chunk_attn_a
     p.window = a->window;
     p.scale = a->scale;
     p.softcap = a->softcap;
+    p.inv_cap = a->softcap > 0.f ? 1.f / a->softcap : 0.f;
+    p.gqa_mul = p.gqa > 1 ? (u32)((1ull << 32) / p.gqa) + 1 : 0;
 }
 
 static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
@@ -648,7 +666,9 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
                 if (pl.seq[1][j].ns > 1) {
                     p.seq[k] = pl.seq[1][j];
                     p.seq[k++].wg0 = (u32)blocks;
-                    blocks += ((u64)pl.seq[1][j].n * p.gqa * L.n_kv_head + per - 1) / per;
+                    const u64 left = (u64)pl.seq[1][j].n * p.gqa - (u64)pl.seq[1][j].cb0 * CK_WCOLS;
+                    const u64 cols = left < (u64)pl.seq[1][j].ncb * CK_WCOLS ? left : (u64)pl.seq[1][j].ncb * CK_WCOLS;
+                    blocks += (cols * L.n_kv_head + per - 1) / per;
                 }
             if (!k) continue;
             p.n_seq = k;

@@ -37,7 +37,7 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
     const u32 ncol = min((u32)CK_COLS, sq.n * p.gqa - c0);
     /* columns past the last one repeat it and are not written */
     const u32 col = c0 + min(i, ncol - 1);
-    const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+    const u32 r = ck_row_of(p, col), head = kvh * p.gqa + col - r * p.gqa;
     const u32 pq = sq.pos + r, end = sq.pos + sq.n;
     const u64 brow = (u64)sq.row + r;
 
@@ -45,7 +45,7 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
     const u32 first = p.first ? p.first[brow] : 0;
     see.set(pq, end, p.window, sq.prefix, first);
     CkSpan span;
-    span.set(sq.pos + c0 / p.gqa, sq.pos + (c0 + ncol - 1) / p.gqa, end, p.window, sq.prefix,
+    span.set(sq.pos + ck_row_of(p, c0), sq.pos + ck_row_of(p, c0 + ncol - 1), end, p.window, sq.prefix,
              p.first ? ck_uniform(group_umin<16>(first)) : 0, p.first ? ck_uniform(group_umax<16>(first)) : 0);
     CkTiles<CK_KEYS> tiles;
     tiles.set(span);
@@ -212,7 +212,7 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
     const __amdgpu_buffer_rsrc_t ra = buf_rsrc(p.ws_acc + part * D);
     const __amdgpu_buffer_rsrc_t rm = buf_rsrc(p.ws_ml + part);
     auto write = [&](u32 c, u32 d, float4 a, float sum, float M) {
-        const u32 cc = c0 + c, rr = cc / p.gqa, hh = kvh * p.gqa + cc % p.gqa;
+        const u32 cc = c0 + c, rr = ck_row_of(p, cc), hh = kvh * p.gqa + cc - rr * p.gqa;
         const u64 br = (u64)sq.row + rr;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         *(float4 *)(p.dst + br * p.q_stride + (u64)hh * D + 4 * d) =
@@ -452,17 +452,18 @@ TL_DEV void ck_wide(const CkAttnParams &p, const CkSeq &sq, CkWideShared<D, Q8> 
     const u32 local = blockIdx.x - sq.wg0;
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 cb = rest % sq.ncb, split = rest / sq.ncb;
-    const u32 cols = sq.n * p.gqa, cw = cb * CK_WCOLS + wave * MC;
+    const u32 cols = sq.n * p.gqa, c0 = (sq.cb0 + cb) * CK_WCOLS, cw = c0 + wave * MC;
     const bool live = cw < cols;
     const u32 col = min(cw + i, cols - 1);
     const u32 end = sq.pos + sq.n;
-    const u32 pq = sq.pos + col / p.gqa, head = kvh * p.gqa + col % p.gqa;
-    const u64 brow = (u64)sq.row + col / p.gqa;
+    const u32 r = ck_row_of(p, col), head = kvh * p.gqa + col - r * p.gqa;
+    const u32 pq = sq.pos + r;
+    const u64 brow = (u64)sq.row + r;
     CkSees see;
     CkSpan span;
     const u32 first = p.first ? p.first[brow] : 0;
     see.set(pq, end, p.window, sq.prefix, first);
-    span.set(sq.pos + min(cw, cols - 1) / p.gqa, sq.pos + min(cw + MC - 1, cols - 1) / p.gqa, end, p.window, sq.prefix,
+    span.set(sq.pos + ck_row_of(p, min(cw, cols - 1)), sq.pos + ck_row_of(p, min(cw + MC - 1, cols - 1)), end, p.window, sq.prefix,
              p.first ? ck_uniform(group_umin<MC>(first)) : 0, p.first ? ck_uniform(group_umax<MC>(first)) : 0);
     u32 fmin = span.fmin, fmax = span.max_f;
     if (p.first) {
@@ -480,7 +481,7 @@ TL_DEV void ck_wide(const CkAttnParams &p, const CkSeq &sq, CkWideShared<D, Q8> 
         fmax = ck_uniform(fmax);
     }
     CkSpan all;
-    all.set(sq.pos + cb * CK_WCOLS / p.gqa, sq.pos + min(cb * CK_WCOLS + CK_WCOLS - 1, cols - 1) / p.gqa, end, p.window,
+    all.set(sq.pos + ck_row_of(p, c0), sq.pos + ck_row_of(p, min(c0 + CK_WCOLS - 1, cols - 1)), end, p.window,
             sq.prefix, fmin, fmax);
     CkTiles<KT> tiles;
     tiles.set(all);
@@ -711,7 +712,8 @@ TL_DEV void ck_wide(const CkAttnParams &p, const CkSeq &sq, CkWideShared<D, Q8> 
                 }
                 score.template apply<SN>(s, (int)(pq - kb - 8 * h), [](int e) { return ck_key<MC>(e); });
                 const u32 bad = (u32)(s_bad[(t - t0) & 3] >> (32 * sub));
-                if (!span.full(kb, 32) || bad) {
+                if (__builtin_expect(!span.full(kb, 32) || bad, 0)) {
+                    asm volatile("");      /* stays a branch: made into selects it cost every tile 18% */
                     u64 keys = 0;
 #pragma unroll
                     for (int w = Q8 ? NW / 2 : 0; w < NW; w++) keys |= s_odd[buf][w];
@@ -729,7 +731,7 @@ TL_DEV void ck_wide(const CkAttnParams &p, const CkSeq &sq, CkWideShared<D, Q8> 
                 for (int e = 1; e < SN; e++) top = fmaxf(top, s[e]);
                 top *= mul;
                 const float thr = m == -INFINITY ? -INFINITY : m + CK_LAZY;
-                if (__any(top > thr)) {
+                if (__builtin_expect(__any(top > thr), 0)) {
                     if constexpr (MC == 16) top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const float mn = top > thr ? top : m;
@@ -841,10 +843,10 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const CkAttnParams p) 
     constexpr u32 V4 = D / 4, CPB = 256 / V4;
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 at = (blockIdx.x - sq.wg0) * CPB + threadIdx.x / V4, d = threadIdx.x % V4;
-    const u32 cols = sq.n * p.gqa;
-    const u32 kvh = at / cols, col = at % cols;
+    const u32 c0 = sq.cb0 * CK_WCOLS, cols = min(sq.n * p.gqa - c0, sq.ncb * CK_WCOLS);
+    const u32 kvh = at / cols;
     if (kvh >= p.c.n_kv) return;
-    const u32 cb = col / CK_WCOLS;
+    const u32 cb = at % cols / CK_WCOLS, col = c0 + at % cols;
     const u64 part = (u64)sq.part0 + (u64)(kvh * sq.ncb + cb) * sq.ns * CK_WCOLS + col % CK_WCOLS;
     float M = -INFINITY, sum = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -876,7 +878,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const CkAttnParams p) 
         }
         M = Mn;
     }
-    const u32 r = col / p.gqa, head = kvh * p.gqa + col % p.gqa;
+    const u32 r = ck_row_of(p, col), head = kvh * p.gqa + col - r * p.gqa;
     const u64 brow = (u64)sq.row + r;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     *(float4 *)(p.dst + brow * p.q_stride + (u64)head * D + 4 * d) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);

@@ -31,13 +31,14 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void chunk_weight_kernel(cons
     const u32 turn = wave / (8 / share);
     const bool real = i < cols;
     const u32 col = real ? i : cols - 1;
-    const u32 pq = sq.pos + col / p.gqa;
-    const u64 brow = (u64)sq.row + col / p.gqa;
+    const u32 r = ck_row_of(p, col);
+    const u32 pq = sq.pos + r;
+    const u64 brow = (u64)sq.row + r;
     const u32 first = p.first ? p.first[brow] : 0;
     CkSees see;
     see.set(pq, end, p.window, sq.prefix, first);
     CkSpan span;
-    span.set(sq.pos, sq.pos + (cols - 1) / p.gqa, end, p.window, sq.prefix,
+    span.set(sq.pos, sq.pos + sq.n - 1, end, p.window, sq.prefix,
              p.first ? ck_uniform(group_umin<16>(first)) : 0, p.first ? ck_uniform(group_umax<16>(first)) : 0);
     auto look = [&](u32 t) -> u32 {
         const u32 key = k0 + t * CK_KEYS + (lane & 31);
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void chunk_weight_kernel(cons
         for (u32 hg = 0; hg < groups; hg++) {
             const u32 kvh = p.c.n_kv >= 8 ? hg * 8 + wave : wave % (8 / share);
             if (kvh >= p.c.n_kv || turn >= share) continue;
-            const u32 head = kvh * p.gqa + col % p.gqa;
+            const u32 head = kvh * p.gqa + col - r * p.gqa;
             CkTile<D, Q8> tile, ahead;
             auto load = [&](CkTile<D, Q8> &to, u32 row) {
                 const u32 rc = row < p.c.cap ? row : 0;
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
     float4 qx[W::QV];
     auto fetch = [&](u32 t) {
         const u32 c = min(t * CT + tc, cols - 1);
-        const u32 r = c / p.gqa, head = kvh * p.gqa + c % p.gqa;
+        const u32 r = ck_row_of(p, c), head = kvh * p.gqa + c - r * p.gqa;
         const float *q = p.q + ((u64)sq.row + r) * p.q_stride + (u64)head * D + 4 * tt;
 #pragma unroll
         for (int j = 0; j < W::QV; j++) qx[j] = *(const float4 *)(q + 4 * W::TPC * j);
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
             *(uint2 *)(s_q[buf][1] + at) = lo;
         }
         if (tt == 0) {
-            const u32 r = c / p.gqa, head = kvh * p.gqa + c % p.gqa, pq = sq.pos + r;
+            const u32 r = ck_row_of(p, c), head = kvh * p.gqa + c - r * p.gqa, pq = sq.pos + r;
             const u64 brow = (u64)sq.row + r;
             const u32 first = p.first ? p.first[brow] : 0;
             CkSees see;
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
                 fmax = ck_uniform(group_umax<32>(f));
             }
             CkSpan span;
-            span.set(sq.pos + cb / p.gqa, sq.pos + min(cb + 31, cols - 1) / p.gqa, end, p.window, sq.prefix, fmin, fmax);
+            span.set(sq.pos + ck_row_of(p, cb), sq.pos + ck_row_of(p, min(cb + 31, cols - 1)), end, p.window, sq.prefix, fmin, fmax);
             if (!span.any(kb, 32)) continue;
             const u32 cl = 32 * sub + i;
             u32 rd = W::at(cl, h);
@@ -301,6 +302,7 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
 #pragma unroll
                 for (int e = 0; e < 16; e++) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e], mul, -lse));
             } else {
+                asm volatile("");      /* stays a branch */
                 const CkSees see = s_see[buf][cl];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
