@@ -9,7 +9,6 @@
 #define CK_KEYS 32             /* keys of one tile */
 #define CK_COLS 16             /* (row, head) columns of a narrow workgroup */
 #define CK_WCOLS 128           /* ... of a wide one */
-#define CK_WKEYS 256           /* keys of a wide workgroup of the attention weight */
 
 /* Split merge: one arrival counter per group, zero between launches, at the
  * start of the workspace; (max, sum) pairs and partial rows follow. */
@@ -17,6 +16,14 @@
 #define CK_CNT_PAD 4
 #define CK_CNT_WORDS (CK_MAX_GROUPS * CK_CNT_PAD)
 static_assert(CK_CNT_WORDS <= TL_MERGE_CNT_WORDS, "counters of a stream's workspace");
+
+/* Keys of a wide workgroup of the attention weight: two blocks of 32 to a wave
+ * halve the work on the columns per key, where they do not cost half of the
+ * waves.  512 rows over 4608 keys, us with one block / two: 32/8/128 f16 91 / 63,
+ * 32/8/64 Q8_0 79 / 53, but 32/8/64 f16 45 / 51 (four waves to a SIMD / two). */
+static constexpr TL_HOSTDEV int ck_weight_keys(int head_dim, bool q8) {
+    return head_dim == 64 ? (q8 ? 512 : 256) : head_dim == 128 && !q8 ? 512 : 256;
+}
 
 /* One chunk of a launch: its workgroups are [wg0, next wg0), ncb column blocks
  * x n_kv heads x ns key splits of them; part0 / grp0: its first partial row

@@ -472,7 +472,7 @@ struct WeightPlan {
     u64 floats;
 };
 
-/* More columns than this keep 256 keys of one head to a workgroup; fewer go
+/* More columns than this keep keys of one head to a workgroup; fewer go
  * through all heads of a run of keys, where reading K is the work. */
 #define CK_WEIGHT_WIDE_MIN CK_COLS
 
@@ -480,6 +480,7 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
                         bool q8, u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.blocks = 0;
     pl.floats = 0;
+    const u32 wkeys = (u32)ck_weight_keys((int)head_dim, q8);
     u64 wgs[2] = {0, 0}, blocks = 0, shares = 0, tiles = 0;
     for (u32 i = 0; i < n; i++) {
         const u64 cols = (u64)ch[i]->n * gqa, end = (u64)ch[i]->pos + ch[i]->n;
@@ -492,8 +493,8 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
             s.part0 = (u32)(lo / CK_KEYS * CK_KEYS);
             tiles += (end - s.part0 + CK_KEYS - 1) / CK_KEYS;
         } else {
-            s.part0 = (u32)(lo / CK_WKEYS * CK_WKEYS);
-            s.ncb = (u32)((end - s.part0 + CK_WKEYS - 1) / CK_WKEYS);
+            s.part0 = (u32)(lo / wkeys * wkeys);
+            s.ncb = (u32)((end - s.part0 + wkeys - 1) / wkeys);
             blocks += s.ncb;
             shares += (u64)s.ncb * ((cols + 127) / 128);
         }
@@ -533,9 +534,9 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
         const u64 parts = ((u64)s.n * gqa + 127) / 128;
         s.ns = (u32)((parts + per - 1) / per);
         s.wg0 = (u32)wgs[1];
-        s.grp0 = (u32)(pl.floats / CK_WKEYS);
+        s.grp0 = (u32)(pl.floats / wkeys);
         wgs[1] += (u64)s.ncb * n_kv * s.ns;
-        pl.floats += (u64)s.ncb * n_kv * s.ns * CK_WKEYS;
+        pl.floats += (u64)s.ncb * n_kv * s.ns * wkeys;
     }
     if (wgs[0] > 0x7fffffffull || wgs[1] > 0x7fffffffull) return false;
     pl.wgs[0] = (u32)wgs[0];
@@ -697,23 +698,24 @@ extern "C" int tl_attn_chunks_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_ar
 /* ------------------------------------------------------------------------ */
 
 /* weight[key] += the sums of the kv heads and column shares, in order */
-__global__ __launch_bounds__(256) void chunk_weight_sum_kernel(const CkAttnParams p) {
+__global__ __launch_bounds__(256) void chunk_weight_sum_kernel(const CkAttnParams p, u32 wkeys) {
     const CkSeq &sq = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
-    const u32 kblk = blockIdx.x - sq.wg0;
-    const u32 key = sq.part0 + kblk * CK_WKEYS + threadIdx.x;
-    if (key >= sq.pos + sq.n) return;
-    const float *in = p.ws_acc + ((u64)sq.grp0 + kblk) * CK_WKEYS + threadIdx.x;
+    /* the sums of a workgroup's keys lie side by side: sets of wkeys */
+    const u32 key = (blockIdx.x - sq.wg0) * 256 + threadIdx.x;
+    const u32 kblk = key / wkeys;
+    if (sq.part0 + key >= sq.pos + sq.n) return;
+    const float *in = p.ws_acc + ((u64)sq.grp0 + kblk) * wkeys + key % wkeys;
     const u32 n = sq.ns * p.c.n_kv;
-    const float old = sq.weight[key];
+    const float old = sq.weight[sq.part0 + key];
     float sum = 0.f;
     for (u32 x = 0; x < n; x += 8) {
         float v[8];
 #pragma unroll
-        for (u32 j = 0; j < 8; j++) v[j] = in[(u64)min(x + j, n - 1) * sq.ncb * CK_WKEYS];
+        for (u32 j = 0; j < 8; j++) v[j] = in[(u64)min(x + j, n - 1) * sq.ncb * wkeys];
 #pragma unroll
         for (u32 j = 0; j < 8; j++) sum += x + j < n ? v[j] : 0.f;
     }
-    sq.weight[key] = old + sum;
+    sq.weight[sq.part0 + key] = old + sum;
 }
 
 static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl_chunk *ch, u32 n_chunk,
@@ -753,10 +755,10 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
             u32 at = 0;
             for (u32 j = 0; j < pl.n[1]; j++) {
                 p.seq[j].wg0 = at;
-                at += p.seq[j].ncb;
+                at += (p.seq[j].pos + p.seq[j].n - p.seq[j].part0 + 255) / 256;
             }
             starts(p);
-            hipLaunchKernelGGL(chunk_weight_sum_kernel, dim3(at), dim3(256), 0, st, p);
+            hipLaunchKernelGGL(chunk_weight_sum_kernel, dim3(at), dim3(256), 0, st, p, (u32)ck_weight_keys((int)L.head_dim, L.q8));
             HIP_TRY(hipGetLastError());
         }
     }

@@ -127,8 +127,8 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void chunk_weight_kernel(cons
 
 /* ---- many columns ------------------------------------------------------------
  *
- * A workgroup keeps 256 keys of one kv head in registers, 32 to a wave, as the A
- * operand of v_mfma_f32_32x32x16_f16, and goes through a share of the head's
+ * A workgroup keeps 512 keys of one kv head in registers (256 where K takes too
+ * many), 64 to a wave, as the A operands of v_mfma_f32_32x32x16_f16, and goes through a share of the head's
  * columns: CT at a time are fetched, split into pairs of f16 and put to LDS by
  * all 512 threads (two buffers, one barrier each), and every wave multiplies its
  * keys with them.  A lane sums 16 keys over one column of 32; the lanes are
@@ -137,8 +137,9 @@ __global__ __launch_bounds__(512, D == 64 ? 4 : 2) void chunk_weight_kernel(cons
  * instructions (two products) and, with capped scores, by the vector ones. */
 typedef float f16w_t __attribute__((ext_vector_type(16)));
 
-template <int D>
+template <int D, bool Q8>
 struct CkWeight {
+    static constexpr int KB = ck_weight_keys(D, Q8) / 256;   /* blocks of 32 keys of a wave */
     static constexpr int CT = D == 256 ? 32 : 64;     /* columns of a buffer */
     static constexpr int TPC = 512 / CT;              /* threads of a column */
     static constexpr int QV = D / 4 / TPC;            /* float4s of one of them */
@@ -151,8 +152,8 @@ struct CkWeight {
 
 template <int D, bool Q8, bool BIAS>
 __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide_kernel(const CkAttnParams p) {
-    typedef CkWeight<D> W;
-    constexpr int NS = D / 16, CT = W::CT;
+    typedef CkWeight<D, Q8> W;
+    constexpr int NS = D / 16, CT = W::CT, KB = W::KB, WKEYS = 256 * KB;
     __shared__ __align__(16) char s_q[2][2][W::PLANE];    /* buffer, hi / lo */
     __shared__ CkScore<BIAS> s_score[2][CT];
     __shared__ CkSees s_see[2][CT];
@@ -166,39 +167,46 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
     const u32 kvh = local % p.c.n_kv, rest = local / p.c.n_kv;
     const u32 kblk = rest % sq.ncb, share = rest / sq.ncb;
     const u32 end = sq.pos + sq.n, cols = sq.n * p.gqa;
-    const u32 kb = sq.part0 + kblk * CK_WKEYS + wave * 32;
+    const u32 k0 = sq.part0 + kblk * WKEYS + wave * (32 * KB);
     const u32 tiles = (cols + CT - 1) / CT;
     const u32 t0 = (u32)((u64)tiles * share / sq.ns), t1 = (u32)((u64)tiles * (share + 1) / sq.ns);
 
     /* matrix row rho is key rho with bits 2 and 3 exchanged (any order would do) */
-    const u32 key = kb + ((i & 19) | ((i & 4) << 1) | ((i & 8) >> 1));
-    const u32 row = key < end ? ck_row(p.c, sq.pages, key) : ~0u;
-    const u32 rc = row < p.c.cap ? row : 0;
-    h8_t kh[NS], kl[Q8 ? NS : 1];
-    if constexpr (!Q8) {
-        const char *base = (const char *)(p.c.k + (u64)kvh * p.c.cap * D);
+    u32 row[KB];
 #pragma unroll
-        for (int s = 0; s < NS; s++) kh[s] = *(const h8_t *)(base + (u64)(rc * (u32)(2 * D) + s * 32 + h * 16));
-    } else {
-        const char *base = (const char *)p.c.k + (u64)kvh * p.c.cap * D;
-        const u16 *sb = p.c.ks + (u64)kvh * p.c.cap * (D / 32);
+    for (int x = 0; x < KB; x++) {
+        const u32 key = k0 + 32 * x + ((i & 19) | ((i & 4) << 1) | ((i & 8) >> 1));
+        row[x] = key < end ? ck_row(p.c, sq.pages, key) : ~0u;
+    }
+    h8_t kh[KB][NS], kl[Q8 ? KB : 1][Q8 ? NS : 1];
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-            const uint2 v = *(const uint2 *)(base + (u64)(rc * (u32)D + s * 16 + h * 8));
-            const tl_half2 d2 = __builtin_bit_cast(tl_half2, (u32)sb[(u64)(rc * (u32)(D / 32) + (s >> 1))] * 0x10001u);
-            tl_half2 x[4];
-            i8x4_to_f16(v.x, x[0], x[1]);
-            i8x4_to_f16(v.y, x[2], x[3]);
-            u4_t a, b;
+    for (int x = 0; x < KB; x++) {
+        const u32 rc = row[x] < p.c.cap ? row[x] : 0;
+        if constexpr (!Q8) {
+            const char *base = (const char *)(p.c.k + (u64)kvh * p.c.cap * D);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                u32 y, z;
-                ck_q8_pair(x[j], d2, y, z);
-                a[j] = y;
-                b[j] = z;
+            for (int s = 0; s < NS; s++) kh[x][s] = *(const h8_t *)(base + (u64)(rc * (u32)(2 * D) + s * 32 + h * 16));
+        } else {
+            const char *base = (const char *)p.c.k + (u64)kvh * p.c.cap * D;
+            const u16 *sb = p.c.ks + (u64)kvh * p.c.cap * (D / 32);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const uint2 v = *(const uint2 *)(base + (u64)(rc * (u32)D + s * 16 + h * 8));
+                const tl_half2 d2 = __builtin_bit_cast(tl_half2, (u32)sb[(u64)(rc * (u32)(D / 32) + (s >> 1))] * 0x10001u);
+                tl_half2 w[4];
+                i8x4_to_f16(v.x, w[0], w[1]);
+                i8x4_to_f16(v.y, w[2], w[3]);
+                u4_t a, b;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    u32 y, z;
+                    ck_q8_pair(w[j], d2, y, z);
+                    a[j] = y;
+                    b[j] = z;
+                }
+                kh[x][s] = __builtin_bit_cast(h8_t, a);
+                kl[x][s] = __builtin_bit_cast(h8_t, b);
             }
-            kh[s] = __builtin_bit_cast(h8_t, a);
-            kl[s] = __builtin_bit_cast(h8_t, b);
         }
     }
 
@@ -247,7 +255,7 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
         }
     };
 
-    float sum[16] = {};
+    float sum[KB][16] = {};
     if (t0 < t1) {
         fetch(t0);
         store(t0);
@@ -269,14 +277,14 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
             }
             CkSpan span;
             span.set(sq.pos + ck_row_of(p, cb), sq.pos + ck_row_of(p, min(cb + 31, cols - 1)), end, p.window, sq.prefix, fmin, fmax);
-            if (!span.any(kb, 32)) continue;
+            if (!span.any(k0, 32 * KB)) continue;
             const u32 cl = 32 * sub + i;
             u32 rd = W::at(cl, h);
             asm volatile("" : "+v"(rd));
             const char *qp = s_q[buf][0];
-            f16w_t s;
+            f16w_t s[KB];
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.f;
+            for (int x = 0; x < KB; x++) s[x] = (f16w_t)(0.f);
             constexpr int AHEAD = 4;
             h8_t a[AHEAD], b[AHEAD];
             auto read = [&](int j) {
@@ -289,39 +297,49 @@ __global__ __launch_bounds__(512, D == 64 && !Q8 ? 4 : 2) void chunk_weight_wide
 #pragma unroll
             for (int j = 0; j < NS; j++) {
                 __builtin_amdgcn_sched_barrier(0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[j], a[j % AHEAD], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[j], b[j % AHEAD], s, 0, 0, 0);
-                if constexpr (Q8) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[j], a[j % AHEAD], s, 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < KB; x++) {
+                    s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[x][j], a[j % AHEAD], s[x], 0, 0, 0);
+                    s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[x][j], b[j % AHEAD], s[x], 0, 0, 0);
+                    if constexpr (Q8) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[x][j], a[j % AHEAD], s[x], 0, 0, 0);
+                }
                 if (j + AHEAD < NS) read(j + AHEAD);
             }
             __builtin_amdgcn_sched_barrier(0);
             const CkScore<BIAS> score = s_score[buf][cl];
             const float mul = score.factor(), lse = s_lse[buf][cl];
-            score.template apply<16>(s, (int)(s_pos[buf][cl] - kb - 8 * h), [](int e) { return 16 * (e >> 3) + (e & 7); });
-            if (span.full(kb, 32)) {
+            const u32 pq = s_pos[buf][cl];
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum[e] += __builtin_amdgcn_exp2f(fmaf(s[e], mul, -lse));
-            } else {
-                asm volatile("");      /* stays a branch */
-                const CkSees see = s_see[buf][cl];
+            for (int x = 0; x < KB; x++) {
+                const u32 kb = k0 + 32 * x;
+                score.template apply<16>(s[x], (int)(pq - kb - 8 * h), [](int e) { return 16 * (e >> 3) + (e & 7); });
+                if (span.full(kb, 32)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const bool v = see.sees(kb + 16 * (e >> 3) + 8 * h + (e & 7));
-                    sum[e] += v ? __builtin_amdgcn_exp2f(fmaf(s[e], mul, -lse)) : 0.f;
+                    for (int e = 0; e < 16; e++) sum[x][e] += __builtin_amdgcn_exp2f(fmaf(s[x][e], mul, -lse));
+                } else {
+                    asm volatile("");      /* stays a branch */
+                    const CkSees see = s_see[buf][cl];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const bool v = see.sees(kb + 16 * (e >> 3) + 8 * h + (e & 7));
+                        sum[x][e] += v ? __builtin_amdgcn_exp2f(fmaf(s[x][e], mul, -lse)) : 0.f;
+                    }
                 }
             }
         }
         if (t + 1 < t1) store(t + 1);
     }
     /* the columns' lanes joined; keys without a row count nothing */
-    const u64 bad = __ballot(row >= p.c.cap);
-    float *out = p.ws_acc + (u64)sq.grp0 * CK_WKEYS +
-                 ((u64)(share * p.c.n_kv + kvh) * sq.ncb + kblk) * CK_WKEYS + wave * 32;
+    float *out = p.ws_acc + ((u64)sq.grp0 + (u64)(share * p.c.n_kv + kvh) * sq.ncb + kblk) * WKEYS + wave * (32 * KB);
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const float x = group_sum<32>(sum[e]);
-        const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
-        const u32 rho = (k & 19) | ((k & 4) << 1) | ((k & 8) >> 1);      /* the lane that holds key k's row */
-        if (i == 0) out[k] = (bad >> rho) & 1 ? 0.f : x;
+    for (int x = 0; x < KB; x++) {
+        const u64 bad = __ballot(row[x] >= p.c.cap);
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float y = group_sum<32>(sum[x][e]);
+            const u32 k = 16 * (e >> 3) + 8 * h + (e & 7);
+            const u32 rho = (k & 19) | ((k & 4) << 1) | ((k & 8) >> 1);      /* the lane that holds key k's row */
+            if (i == 0) out[32 * x + k] = (bad >> rho) & 1 ? 0.f : y;
+        }
     }
 }
