@@ -384,7 +384,7 @@ typedef struct tl_chunk {
  *     y = x / sqrt(mean(x^2) + eps) * weight      over each head's head_dim
  * for every head of q and k, then the rotation `rope` (as tl_rope_params, the
  * angle reduced in 64 bits), q to q_out, and the new K and V rows into the
- * cache (V as it is).  q_out may be q. */
+ * cache (V as it is).  q_out may be q, or share no floats with q, k and v. */
 typedef struct tl_qk_norm_args {
     const float *q;           /* device [rows][q_stride] */
     const float *k;           /* device [rows][kv_stride] */
@@ -415,8 +415,9 @@ int tl_qk_norm_append_q8(const tl_kv_layer_q8 *L, const tl_qk_norm_args *a,
  *     s = scale * q.k;  softcap > 0: s = softcap * tanh(s / softcap)
  *     slopes: s -= slopes[head] * |p - j|
  * A row that sees nothing gives zeros, and a log sum of -infinity.  Keys that
- * a row does not see have no part in it, whatever their K and V hold; a key
- * that it does see should be finite. */
+ * a row does not see have no part in it, whatever their K and V hold; one that
+ * sees an infinity or NaN may come out as NaN (a Q8_0 element counts as an
+ * infinity past the range of f16).  dst shares no floats with q. */
 typedef struct tl_chunk_attn_args {
     const float    *q;        /* device [rows][q_stride], rotated */
     float          *dst;      /* device [rows][q_stride] */
@@ -431,7 +432,7 @@ typedef struct tl_chunk_attn_args {
     uint32_t        page_size;
     uint32_t        window;   /* 0 = all */
     float           scale;    /* > 0 */
-    float           softcap;  /* 0 = none */
+    float           softcap;  /* 0 = none, else at least 1e-6 */
     void           *ws;       /* device workspace of this call, 16-byte aligned, zeroed before its
                                  first use and used by one call at a time; NULL = the stream's
                                  own (not under HIP graph capture) */

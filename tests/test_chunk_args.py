@@ -65,7 +65,7 @@ def test_chunks_refused(name, cs, code):
     dict(slopes=P + 3), dict(n_head=0), dict(n_head=12), dict(q_stride=4092), dict(q_stride=4098),
     dict(page_size=0), dict(page_size=24), dict(page_size=8192), dict(scale=0.0), dict(scale=-1.0),
     dict(scale=float("nan")), dict(scale=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")),
-    dict(softcap=float("inf")), dict(ws=P + 8), dict(dst=1 << 30), dict(dst=(1 << 30) + 4096 * 16)])
+    dict(softcap=float("inf")), dict(softcap=1e-7), dict(ws=P + 8), dict(dst=1 << 30), dict(dst=(1 << 30) + 4096 * 16)])
 def test_attn_args_refused(bad):
     L, (ch, n) = tlkv.lib(), chunks(ONE)
     assert L.tl_attn_chunks(layer(), attn(**bad), ch, n, None) == -1
@@ -89,7 +89,8 @@ def test_attn_workspace_refused():
     dict(kv_stride=1026), dict(q_out_stride=4000), dict(page_size=3), dict(eps=-1.0), dict(eps=float("nan")),
     dict(eps=float("inf")), dict(rope=tlkv.RopeParams(130, 1e4, 0)), dict(rope=tlkv.RopeParams(63, 1e4, 0)),
     dict(rope=tlkv.RopeParams(64, 0.0, 0)), dict(rope=tlkv.RopeParams(64, float("inf"), 0)),
-    dict(q_out=(1 << 30) + 16), dict(q_out=1 << 30, q_out_stride=4100)])
+    dict(q_out=(1 << 30) + 16), dict(q_out=1 << 30, q_out_stride=4100), dict(q_out=5 * P, k=5 * P + 4096 * 8),
+    dict(q_out=6 * P + 16), dict(q=1 << 30, q_stride=6144, q_out_stride=6144, q_out=(1 << 30) + 2064 * 4)])
 def test_norm_args_refused(bad):
     L, (ch, n) = tlkv.lib(), chunks(ONE)
     assert L.tl_qk_norm_append(layer(), norm(**bad), ch, n, None) == -1
@@ -116,6 +117,14 @@ def test_weight_refused():
         ch, n = chunks(*cs)
         assert L.tl_attn_weight(layer(), a, ch, n, None) == -1
         assert L.tl_attn_weight_q8(layer_q8(), a, ch, n, None) == -1
+
+
+def test_too_many_columns_refused():
+    """Rows x gqa^2 past 32 bits: the kernels divide by multiplication."""
+    L, (ch, n) = tlkv.lib(), chunks(dict(n=1 << 20, row=0))
+    for name in ("tl_attn_chunks", "tl_attn_weight"):
+        a = attn(rows=1 << 20, n_head=512, q_stride=65536, dst=1 << 45)
+        assert getattr(L, name)(layer(), a, ch, n, None) == -2
 
 
 def test_nothing_to_do():

@@ -12,7 +12,8 @@ import chunk_ref as R
 pytestmark = pytest.mark.gpu
 
 SHAPES = {"1b": (32, 8, 64), "8b": (32, 8, 128), "qwen": (28, 4, 128), "gemma": (8, 4, 256),
-          "mha": (8, 8, 128), "mqa": (20, 1, 64)}
+          "mha": (8, 8, 128), "mqa": (20, 1, 64), "kv12": (12, 12, 64), "kv3": (9, 3, 128),
+          "mqa40": (40, 1, 128)}
 
 
 @pytest.fixture(scope="module")
@@ -131,6 +132,15 @@ ATTN = [
     ("gemma", [(77, 140)], 16, False, dict(window=64)),
     ("8b", [(513, 129)], 16, True, dict(window=300, prefix=[600])),
     ("mqa", [(11, 60)], 16, False, {}),
+    ("kv12", [(100, 1), (3, 2), (70, 40)], 16, False, dict(window=33)),
+    ("kv3", [(300, 1), (3, 2), (70, 4)], 16, True, dict(softcap=10.0)),
+    ("mqa40", [(40, 1), (3, 2)], 16, False, dict(prefix=[9, 2])),
+    ("8b", [(40, 60), (700, 1), (0, 3), (1300, 2)], 16, True, dict(slopes=True)),
+    ("1b", [(0, 200), (2000, 1), (31, 16)], 16, False, dict(first=True, window=90)),
+    ("gemma", [(0, 1), (600, 70), (1200, 1)], 16, True, dict(prefix=[0, 300, 7])),
+    ("qwen", [(700, 300)], 64, False, dict(window=200, prefix=[100])),
+    ("8b", [(0, 400)], 16, False, {}),
+    ("mha", [(1000, 140), (20, 17)], 1, True, dict(softcap=20.0, first=True)),
 ]
 
 
@@ -206,6 +216,8 @@ def test_attn_chunks_unseen_rows_hold_anything(T, q8, n, pos):
     if n > 1:
         ok[n - 1] = False      # sees the spoilt position
     assert np.isfinite(dst[ok]).all()
+    if n > 1:
+        assert not np.isfinite(dst[n - 1]).all()
     assert rel(dst[ok], want[0][ok]) <= want[2]
     assert np.abs(lse[ok] - want[1][ok]).max() <= want[2] + 4 * R.U24 * 10
 
@@ -361,6 +373,77 @@ def test_attn_weight_unseen_rows_hold_anything(T):
     got = w[0].cpu().numpy()
     assert np.isfinite(got).all() and np.all(got[[0, 1, 42]] == 0)
     assert abs(got.sum() - 2 * B.H) < 1e-3
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attn_and_weight_share_a_workspace_in_a_graph(T, q8):
+    """One workspace for the attention and the weight of a step, captured together and replayed
+    with eager calls between: every replay equals the eager step."""
+    B = R.Batch(37, SHAPES["8b"], [(2500, 1), (300, 70), (40, 3)], 16, q8)
+    D = Dev(T, B)
+    scale = 1 / math.sqrt(B.D)
+    w = [T.zeros(p + n, device="cuda") for p, n in B.sizes]
+    ch = D.chunks(weight=w)
+    ws = ws_of(T, D, D.attn_args(scale), ch)
+    args = D.attn_args(scale, ws=ws)
+    D.attn(scale)
+    D.call("tl_attn_weight", D.attn_args(scale), ch)
+    T.cuda.synchronize()
+    base = [x.clone() for x in w]
+    out = D.dst.clone()
+    s = T.cuda.Stream()
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g, stream=s):
+        h = D.t.stream_handle(s)
+        D.call("tl_attn_chunks", args, ch, h)
+        D.call("tl_attn_weight", args, ch, h)
+    for _ in range(3):
+        for x in w + [D.dst, D.lse]:
+            x.zero_()
+        g.replay()
+        T.cuda.synchronize()
+        m = real_rows(B)
+        assert all(T.equal(a, b) for a, b in zip(w, base))
+        assert np.array_equal(D.dst.cpu().numpy()[m], out.cpu().numpy()[m])
+        D.attn(scale)
+    with T.cuda.graph(T.cuda.CUDAGraph(), stream=s):
+        with pytest.raises(D.t.TlError, match="workspace"):
+            D.call("tl_attn_weight", D.attn_args(scale), ch, D.t.stream_handle(s))
+        D.dst.fill_(1.0)
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_pool_of_four_gib_per_head(T, n):
+    """Rows at the end of the largest pool that a layer may have: offsets within a head pass 31
+    bits, the heads' bases 32."""
+    H, KV, Dm = 4, 2, 128
+    cap = (1 << 32) // (Dm * 2) - 16
+    sizes = [(90, n)]
+    B = R.Batch(41, (H, KV, Dm), sizes, 16, spare=0)
+    pages = -(-(90 + n) // 16)
+    k = T.empty((KV, cap, Dm), dtype=T.float16, device="cuda")
+    v = T.empty_like(k)
+    D = Dev(T, B)
+    small, B.cap = B.tables[0].copy(), cap
+    B.tables[0] = (cap // 16 - 1 - np.arange(pages)).astype(np.uint32)
+    far = T.from_numpy(B.phys(0, np.arange(90 + n))).cuda()
+    near = T.from_numpy((small[np.arange(90 + n) // 16].astype(np.int64) * 16 + np.arange(90 + n) % 16)).cuda()
+    k[:, far], v[:, far] = D.x["k"][:, near], D.x["v"][:, near]
+    D.tab = [T.from_numpy(B.tables[0].view(np.int32)).cuda()]
+    D.layer = D.t.KvLayer(k.data_ptr(), v.data_ptr(), cap, KV, Dm, 0)
+    B.tables[0], B.cap = small, pages * 16
+    want = R.attn(B, 0.1)
+    got = D.attn(0.1)
+    check_attn(B, got, want)
+    w = [T.zeros(90 + n, device="cuda")]
+    D.call("tl_attn_weight", D.attn_args(0.1), D.chunks(weight=w))
+    a = D.t.QkNormArgs(q=D.x["q"].data_ptr(), k=D.x["kin"].data_ptr(), v=D.x["vin"].data_ptr(),
+                       q_out=D.dst.data_ptr(), eps=1e-6, rows=B.rows, n_head=H, q_stride=B.q_stride,
+                       kv_stride=B.kv_stride, q_out_stride=B.q_stride, page_size=16)
+    D.call("tl_qk_norm_append", a, D.chunks())
+    T.cuda.synchronize()
+    assert abs(float(w[0].sum()) - n * H) <= 1e-3 * n * H
+    assert T.equal(v[:, far[90:]].cpu(), T.from_numpy(B.vin[:n].reshape(n, KV, Dm).transpose(1, 0, 2).astype(np.float16)))
 
 
 # ---- norm + rotation + append --------------------------------------------------------

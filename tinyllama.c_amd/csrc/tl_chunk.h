@@ -457,7 +457,7 @@ struct CkScore {
     bool capped, sloped;
     /* cs: factor from the products to scale * q.k */
     TL_DEV void set(const CkAttnParams &p, float cs, u32 head) {
-        mul = cs * CK_LOG2E;
+        mul = fmaxf(cs * CK_LOG2E, 1.1754944e-38f);      /* not zero: hidden scores are -infinity x mul */
         if constexpr (BIAS) {
             capped = p.softcap > 0.f;
             sloped = p.slopes != nullptr;

@@ -101,6 +101,17 @@ static u64 span(u32 rows, u32 stride, u32 width) {
     return rows ? ((u64)(rows - 1) * stride + width) * sizeof(float) : 0;
 }
 
+/* Do the rows of two buffers share floats?  Buffers of one stride may lie side
+ * by side in each row (q, k and v of one projection). */
+static bool rows_overlap(u32 rows, const float *a, u32 a_stride, u32 a_width, const float *b, u32 b_stride,
+                         u32 b_width) {
+    if (!tl_ranges_overlap(a, span(rows, a_stride, a_width), b, span(rows, b_stride, b_width))) return false;
+    if (a_stride != b_stride) return true;
+    const long long d = b - a, s = a_stride;
+    const u64 at = (u64)((d % s + s) % s);      /* column of b in a's rows */
+    return at < a_width || at + b_width > a_stride;
+}
+
 static int check_rows(const char *what, const void *p, u32 stride, u64 width) {
     if (!p) return tl_fail(TL_EINVAL, "chunks: null %s", what);
     if (stride < width || (stride & 3) || ((uintptr_t)p & 15))
@@ -249,14 +260,11 @@ static int norm_append(const LayerView &L, const tl_qk_norm_args *a, const tl_ch
     if (((uintptr_t)a->q_weight | (uintptr_t)a->k_weight) & 15)
         return tl_fail(TL_EINVAL, "qk_norm: weights not 16-byte aligned");
     if (!(a->eps >= 0.f) || !isfinite(a->eps)) return tl_fail(TL_EINVAL, "qk_norm: eps %g", (double)a->eps);
-    if (a->q_out == a->q ? a->q_out_stride != a->q_stride
-                         : tl_ranges_overlap(a->q, span(a->rows, a->q_stride, (u32)qw), a->q_out,
-                                             span(a->rows, a->q_out_stride, (u32)qw)) &&
-                               /* column blocks of one buffer lie apart in each row */
-                               !(a->q_stride == a->q_out_stride &&
-                                 (u64)((a->q > a->q_out ? a->q - a->q_out : a->q_out - a->q)) >= qw &&
-                                 (u64)((a->q > a->q_out ? a->q - a->q_out : a->q_out - a->q)) + qw <= a->q_stride))
-        return tl_fail(TL_EINVAL, "qk_norm: q_out overlaps q");
+    const bool place = a->q_out == a->q && a->q_out_stride == a->q_stride;
+    if ((!place && rows_overlap(a->rows, a->q, a->q_stride, (u32)qw, a->q_out, a->q_out_stride, (u32)qw)) ||
+        rows_overlap(a->rows, a->k, a->kv_stride, (u32)kw, a->q_out, a->q_out_stride, (u32)qw) ||
+        rows_overlap(a->rows, a->v, a->kv_stride, (u32)kw, a->q_out, a->q_out_stride, (u32)qw))
+        return tl_fail(TL_EINVAL, "qk_norm: q_out overlaps q, k or v");
     RopeCfg rope;
     rope.rdim = 0;
     if (a->rope.rope_dim) {
@@ -431,7 +439,8 @@ static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_
     if (rc) return rc;
     if (((uintptr_t)a->lse | (uintptr_t)a->first | (uintptr_t)a->slopes) & 3)
         return tl_fail(TL_EINVAL, "attn_chunks: lse, first or slopes not aligned");
-    if (!(a->scale > 0.f) || !isfinite(a->scale) || !(a->softcap >= 0.f) || !isfinite(a->softcap))
+    if (!(a->scale > 0.f) || !isfinite(a->scale) || !(a->softcap == 0.f || a->softcap >= 1e-6f) ||
+        !isfinite(a->softcap))
         return tl_fail(TL_EINVAL, "attn_chunks: scale %g softcap %g", (double)a->scale, (double)a->softcap);
     const u64 gqa = a->n_head / L.n_kv_head;
     for (u32 i = 0; i < n_chunk; i++)
@@ -624,8 +633,8 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
     u32 shift;
     int rc = check_attn(L, a, ch, n_chunk, false, &shift);
     if (rc) return rc;
-    if (tl_ranges_overlap(a->q, span(a->rows, a->q_stride, a->n_head * L.head_dim), a->dst,
-                          span(a->rows, a->q_stride, a->n_head * L.head_dim)))
+    const u32 width = a->n_head * L.head_dim;
+    if (rows_overlap(a->rows, a->q, a->q_stride, width, a->dst, a->q_stride, width))
         return tl_fail(TL_EINVAL, "attn_chunks: dst overlaps q");
     CkAttnParams p;
     fill_attn(p, L, a, shift);
