@@ -348,23 +348,60 @@ struct AttnPlan {
     u32 groups;                 /* merge counters (narrow) */
 };
 
-/* More columns than this take the wide kernel. */
+/* Chunks of more columns than this take the wide kernel, unless the whole batch
+ * is cheaper on the narrow one.  Its cost (us) is a round of up to 256 groups at a
+ * time plus a time per 1000 tiles of 32 keys x 16 columns; the wide kernel's a
+ * start (with the join of its splits) plus a time per 1000 tiles of 32 keys x 128
+ * columns.  Fitted to both sides of 70 shapes; us narrow / wide at 32/8/128: 9
+ * rows at 6000 keys 17 / 34, 60 rows 36 / 38, 200 rows 117 / 62; 128 rows at 500
+ * keys 13 / 24; a first prompt of 300 rows 24 / 22; 8 sessions of 100 rows at 1000
+ * keys 103 / 54. */
 #define CK_WIDE_MIN 32
+struct AttnCost {
+    float base, round, tile;     /* narrow */
+    float start, wtile;          /* wide */
+};
+static const AttnCost g_attn_cost[3][2] = {
+    /* f16, Q8_0 */
+    {{2.f, 4.f, 0.78f, 17.f, 2.8f}, {2.f, 4.f, 0.87f, 19.f, 3.4f}},       /* head_dim 64 */
+    {{3.f, 5.5f, 1.2f, 23.f, 3.6f}, {3.f, 5.5f, 1.5f, 24.f, 5.4f}},       /* 128 */
+    {{10.f, 5.f, 3.2f, 22.f, 9.f}, {10.f, 5.f, 3.9f, 25.f, 11.f}},        /* 256 */
+};
+
+/* all of the batch on the narrow kernel? */
+static bool all_narrow(const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim, bool q8, u32 window) {
+    const AttnCost &c = g_attn_cost[head_dim == 64 ? 0 : head_dim == 128 ? 1 : 2][q8];
+    double groups = 0, small = 0, big = 0, wide = 0;
+    for (u32 i = 0; i < n; i++) {
+        const u64 cols = (u64)ch[i]->n * gqa;
+        const u32 step = (CK_COLS + gqa - 1) / gqa, rows = ch[i]->n;
+        /* keys of the first and the last column block, on average */
+        const double keys = 0.5e-3 * n_kv * (double)(span_tiles(*ch[i], window, 0, step < rows ? step : rows) +
+                                                     span_tiles(*ch[i], window, rows > step ? rows - step : 0, rows));
+        groups += (double)n_kv * ((cols + CK_COLS - 1) / CK_COLS);
+        (cols > CK_WIDE_MIN ? big : small) += keys * ((cols + CK_COLS - 1) / CK_COLS);
+        if (cols > CK_WIDE_MIN) wide += keys * ((cols + CK_WCOLS - 1) / CK_WCOLS);
+    }
+    if (big == 0) return true;
+    return c.base + c.round * ceil(groups / 256) + c.tile * (small + big) <=
+           c.start + c.wtile * wide + 0.6 * c.tile * small;
+}
 
 /* As many splits as fill the chip (narrow: one workgroup to a CU, wide: two, at
  * head_dim 256 one; in one launch of both, up to head_dim 128, the narrow ones
  * are of half the size and take what the wide ones leave), none of fewer tiles
  * than a narrow workgroup has waves, or of fewer keys than 128 (wide). */
-static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim,
+static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim, bool q8,
                       u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
     pl.parts = 0;
     u64 tiles[2][CK_MAX_SEQ], total[2] = {0, 0};
+    const u64 wide_min = all_narrow(ch, n, n_kv, gqa, head_dim, q8, window) ? ~0ull : CK_WIDE_MIN;
     u32 n_wide = 0;
-    for (u32 i = 0; i < n; i++) n_wide += (u64)ch[i]->n * gqa > CK_WIDE_MIN;
+    for (u32 i = 0; i < n; i++) n_wide += (u64)ch[i]->n * gqa > wide_min;
     for (u32 i = 0; i < n; i++) {
         const u64 cols = (u64)ch[i]->n * gqa;
-        const int w = cols > CK_WIDE_MIN;
+        const int w = cols > wide_min;
         const u32 per = w ? CK_WCOLS : CK_COLS;
         const u32 ncb = (u32)((cols + per - 1) / per);
         /* bands of a wide chunk, each with splits by its own keys: its last rows see
@@ -459,7 +496,7 @@ static u32 next_chunks(const tl_chunk *ch, u32 n_chunk, u32 *at, const tl_chunk 
 }
 
 /* most partial rows that the attention's launches of one group of chunks take */
-static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, u32 window, const tl_chunk *ch, u32 n_chunk,
+static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, bool q8, u32 window, const tl_chunk *ch, u32 n_chunk,
                        u64 *parts) {
     AttnPlan pl;
     const tl_chunk *of[CK_MAX_SEQ];
@@ -467,7 +504,7 @@ static bool most_parts(u32 n_kv, u32 gqa, u32 head_dim, u32 window, const tl_chu
     for (u32 i = 0; i < n_chunk;) {
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        if (!plan_attn(pl, of, m, n_kv, gqa, head_dim, window)) return false;
+        if (!plan_attn(pl, of, m, n_kv, gqa, head_dim, q8, window)) return false;
         *parts = pl.parts > *parts ? pl.parts : *parts;
     }
     return true;
@@ -573,12 +610,13 @@ extern "C" int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl
     if (!a || !bytes || (n_chunk && !chunks) || n_chunk > CK_MAX_CHUNKS || !n_kv_head || !a->n_head ||
         a->n_head % n_kv_head || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return tl_fail(TL_EINVAL, "attn_chunks_ws: arguments");
-    u64 parts, floats[2];
-    if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, a->window, chunks, n_chunk, &parts) ||
+    u64 parts[2], floats[2];
+    if (!most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, false, a->window, chunks, n_chunk, &parts[0]) ||
+        !most_parts(n_kv_head, a->n_head / n_kv_head, head_dim, true, a->window, chunks, n_chunk, &parts[1]) ||
         !most_sums(n_kv_head, a->n_head / n_kv_head, head_dim, false, a->window, chunks, n_chunk, &floats[0]) ||
         !most_sums(n_kv_head, a->n_head / n_kv_head, head_dim, true, a->window, chunks, n_chunk, &floats[1]))
         return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
-    const u64 attn = ws_need(parts, head_dim), weight = CK_WS_HEAD + (floats[0] > floats[1] ? floats[0] : floats[1]) * sizeof(float);
+    const u64 attn = ws_need(parts[0] > parts[1] ? parts[0] : parts[1], head_dim), weight = CK_WS_HEAD + (floats[0] > floats[1] ? floats[0] : floats[1]) * sizeof(float);
     *bytes = attn > weight ? attn : weight;
     return TL_OK;
 }
@@ -639,7 +677,7 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
     CkAttnParams p;
     fill_attn(p, L, a, shift);
     u64 parts;
-    if (!most_parts(L.n_kv_head, p.gqa, L.head_dim, a->window, ch, n_chunk, &parts))
+    if (!most_parts(L.n_kv_head, p.gqa, L.head_dim, L.q8, a->window, ch, n_chunk, &parts))
         return tl_fail(TL_ERANGE, "attn_chunks: too many workgroups");
     rc = take_ws(a, parts, parts * L.head_dim, st, p);
     if (rc) return rc;
@@ -648,7 +686,7 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
     for (u32 i = 0; i < n_chunk;) {
         const u32 m = next_chunks(ch, n_chunk, &i, of);
         if (!m) break;
-        plan_attn(pl, of, m, L.n_kv_head, p.gqa, L.head_dim, a->window);
+        plan_attn(pl, of, m, L.n_kv_head, p.gqa, L.head_dim, L.q8, a->window);
         const bool both = pl.n[0] && pl.n[1] && L.head_dim != 256;
         for (int w = 1; w >= (both ? 1 : 0); w--) {
             if (!pl.wgs[w]) continue;
