@@ -303,6 +303,31 @@ def test_attn_chunks_repeats_and_graphs(T, q8):
         D.dst.fill_(1.0)
 
 
+@pytest.mark.parametrize("shape,sizes,q8,opt", [
+    ("gemma", [(5000, 8)], False, {}),
+    ("gemma", [(9000, 1), (4000, 3)], True, dict(softcap=30.0)),
+    ("qwen", [(6001, 2)], False, dict(slopes=True)),
+    ("qwen", [(9000, 1)], True, dict(first=True)),
+    ("1b", [(12000, 4)], False, dict(window=9000, prefix=[50])),
+    ("mqa", [(2500, 2)], False, {}),
+])
+def test_attn_chunks_many_splits(T, shape, sizes, q8, opt):
+    """One session whose keys are dealt out to many workgroups: joined in two steps, with the same
+    bits every time, and every counter of the workspace back at zero."""
+    B = R.Batch(23, SHAPES[shape], sizes, 16, q8)
+    D = Dev(T, B)
+    scale = 1 / math.sqrt(B.D)
+    kw = options(B, opt)
+    base = D.attn(scale, prefix=opt.get("prefix"), **kw)
+    check_attn(B, base, R.attn(B, scale, prefix=opt.get("prefix"), **kw))
+    ws = ws_of(T, D, D.attn_args(scale, **kw), D.chunks(opt.get("prefix")))
+    for _ in range(3):
+        D.dst.fill_(7.5)
+        again = D.attn(scale, prefix=opt.get("prefix"), ws=ws, **kw)
+        assert all(np.array_equal(a, b) for a, b in zip(base, again))
+        assert not ws[:65536].any()
+
+
 def test_attn_chunks_two_streams(T):
     """Calls on two streams at once do not share partials."""
     scale = 1 / math.sqrt(128)

@@ -10,11 +10,25 @@
 #define CK_COLS 16             /* (row, head) columns of a narrow workgroup */
 #define CK_WCOLS 128           /* ... of a wide one */
 
-/* Split merge: one arrival counter per group, zero between launches, at the
+/* waves of a narrow workgroup: one workgroup to a CU; four in a launch of both kinds */
+#define CK_WAVES(D) ((D) == 256 ? 4 : 8)
+
+/* Split merge: arrival counters of the groups, zero between launches, at the
  * start of the workspace; (max, sum) pairs and partial rows follow. */
 #define CK_MAX_GROUPS 4096
 #define CK_CNT_PAD 4
 #define CK_CNT_WORDS (CK_MAX_GROUPS * CK_CNT_PAD)
+/* Counters of a group of ns splits of `cols` columns in workgroups of `waves`:
+ * its own and, where one workgroup would wait for memory twice or more to read
+ * them all (eight float4s of a thread at a time), one for each CK_JOIN splits that
+ * are joined first.  One join / joins of eight, us: 16 columns of 256 at 30000 keys
+ * 98.9 / 49.9, 14 of 128 at 16000 keys 32.0 / 17.0; where one wait suffices, 4 of 128
+ * at 6000 keys, 13.1 / 13.8. */
+#define CK_JOIN 8
+static constexpr TL_HOSTDEV u32 ck_join_counters(u32 ns, u32 cols, u32 head_dim, u32 waves) {
+    const u32 units = (cols < CK_COLS ? cols : CK_COLS) * (head_dim / 4);
+    return ns > CK_JOIN && (u64)ns * units >= 2 * 8 * 64 * waves ? 1 + (ns + CK_JOIN - 1) / CK_JOIN : 1;
+}
 static_assert(CK_CNT_WORDS <= TL_MERGE_CNT_WORDS, "counters of a stream's workspace");
 
 /* Keys of a wide workgroup of the attention weight: two blocks of 32 to a wave
@@ -35,6 +49,7 @@ struct CkSeq {
     u32 wg0, ncb, ns, part0, grp0;   /* part0 counts columns */
     u32 wide;                        /* in a launch of both kinds: 128 columns to a workgroup */
     u32 cb0;                         /* wide: its first column block (a band of the chunk's) */
+    u32 counters;                    /* narrow: of one group */
 };
 
 struct CkCache {

@@ -345,7 +345,7 @@ struct AttnPlan {
     CkSeq seq[2][CK_MAX_SEQ];   /* [0]: narrow, [1]: wide */
     u32 n[2], wgs[2];
     u64 parts;                  /* partial rows */
-    u32 groups;                 /* merge counters (narrow) */
+    u32 groups;                 /* their counters (narrow) */
 };
 
 /* Chunks of more columns than this take the wide kernel, unless the whole batch
@@ -371,19 +371,23 @@ static const AttnCost g_attn_cost[3][2] = {
 /* all of the batch on the narrow kernel? */
 static bool all_narrow(const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim, bool q8, u32 window) {
     const AttnCost &c = g_attn_cost[head_dim == 64 ? 0 : head_dim == 128 ? 1 : 2][q8];
-    double groups = 0, small = 0, big = 0, wide = 0;
+    double groups = 0, small = 0, big = 0, wide = 0, most = 0;
     for (u32 i = 0; i < n; i++) {
         const u64 cols = (u64)ch[i]->n * gqa;
         const u32 step = (CK_COLS + gqa - 1) / gqa, rows = ch[i]->n;
         /* keys of the first and the last column block, on average */
         const double keys = 0.5e-3 * n_kv * (double)(span_tiles(*ch[i], window, 0, step < rows ? step : rows) +
                                                      span_tiles(*ch[i], window, rows > step ? rows - step : 0, rows));
+        const double last = 1e-3 * (double)span_tiles(*ch[i], window, 0, rows);
         groups += (double)n_kv * ((cols + CK_COLS - 1) / CK_COLS);
+        most = last > most ? last : most;
         (cols > CK_WIDE_MIN ? big : small) += keys * ((cols + CK_COLS - 1) / CK_COLS);
         if (cols > CK_WIDE_MIN) wide += keys * ((cols + CK_WCOLS - 1) / CK_WCOLS);
     }
     if (big == 0) return true;
-    return c.base + c.round * ceil(groups / 256) + c.tile * (small + big) <=
+    /* more than a round of groups of unequal lengths: the last one to start is late */
+    const double late = groups > 256 ? 128 * most : 0;
+    return c.base + c.round * ceil(groups / 256) + c.tile * (small + big + late) <=
            c.start + c.wtile * wide + 0.6 * c.tile * small;
 }
 
@@ -442,15 +446,19 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
             CkSeq &s = pl.seq[w][i];
             u64 ns = (tiles[w][i] + per - 1) / per;
             const u64 groups = (u64)s.ncb * n_kv;
-            if (ns < 1 || (!w && pl.groups + groups > CK_MAX_GROUPS)) ns = 1;
+            const u64 cols = (u64)s.n * gqa;
+            const u32 counters = ck_join_counters((u32)ns, cols < CK_COLS ? (u32)cols : CK_COLS, head_dim,
+                                            both ? 4 : CK_WAVES(head_dim));
+            if (ns < 1 || (!w && pl.groups + groups * counters > CK_MAX_GROUPS)) ns = 1;
             s.ns = (u32)ns;
+            s.counters = counters;
             s.wg0 = (u32)wgs;
             s.part0 = (u32)pl.parts;
             s.grp0 = pl.groups;
             wgs += groups * ns;
             if (ns > 1) {
                 pl.parts += groups * ns * (w ? CK_WCOLS : CK_COLS);
-                if (!w) pl.groups += (u32)groups;
+                if (!w) pl.groups += (u32)(groups * counters);
             }
         }
         if (wgs > 0x7fffffffull || pl.parts > 0xffffffffull) return false;

@@ -6,9 +6,6 @@
 #pragma once
 #include "tl_chunk.h"
 
-/* waves of a narrow workgroup: one workgroup to a CU */
-#define CK_WAVES(D) ((D) == 256 ? 4 : 8)
-
 /* the maximum moves only when a score passes it by more than 2^CK_LAZY, and
  * probabilities are taken against 2^CK_UP below it: they reach 2^15 at most, so
  * that the low halves of the small ones stay normal f16 numbers too */
@@ -221,6 +218,14 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
             p.lse[br * p.n_head + hh] = sum == 0.f ? -INFINITY
                 : ((M == -INFINITY ? 0.f : M) - CK_UP + __builtin_amdgcn_logf(sum)) * CK_LN2;
     };
+    auto keep = [&](u32 s, u32 c, u32 d, float4 a, float sum, float M) {
+        const u32x4v_t v = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(a.z), __float_as_uint(a.w)};
+        __builtin_amdgcn_raw_buffer_store_b128(v, ra, ((s * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
+        if (d == 0) {
+            const u32x2v_t ml = {__float_as_uint(M), __float_as_uint(sum)};
+            __builtin_amdgcn_raw_buffer_store_b64(ml, rm, (s * CK_COLS + c) * 8, 0, TL_SC1);
+        }
+    };
     for (u32 u = threadIdx.x; u < units; u += NT) {
         const u32 c = u / V4, d = u % V4;
         float M = -INFINITY;
@@ -239,82 +244,83 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
             a.z = fmaf(f, v.z, a.z);
             a.w = fmaf(f, v.w, a.w);
         }
-        if (sq.ns == 1) {
-            write(c, d, a, sum, M);
-        } else {
-            const u32x4v_t v = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(a.z), __float_as_uint(a.w)};
-            __builtin_amdgcn_raw_buffer_store_b128(v, ra, ((split * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
-            if (d == 0) {
-                const u32x2v_t ml = {__float_as_uint(M), __float_as_uint(sum)};
-                __builtin_amdgcn_raw_buffer_store_b64(ml, rm, (split * CK_COLS + c) * 8, 0, TL_SC1);
-            }
-        }
+        if (sq.ns == 1) write(c, d, a, sum, M);
+        else keep(split, c, d, a, sum, M);
     }
     if (sq.ns == 1) return;
-    /* the last split of the group to arrive joins them all: `parts` threads to
-     * a float4 of the output, each with a run of the splits, eight of them
-     * requested at a time; then the parts through LDS, in order */
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    u32 *cnt = p.cnt + (u64)(sq.grp0 + group) * CK_CNT_PAD;
-    if (threadIdx.x == 0)
-        sh.last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == sq.ns - 1;
-    __syncthreads();
-    if (!sh.last) return;
-    u32 parts = 1;
-    while (parts < NW && parts * 2 * units <= NT && parts * 8 < sq.ns) parts *= 2;
-    const u32 run = (sq.ns + parts - 1) / parts;
-    const u32 lanes = parts == 1 ? NT : NT / parts;
-    const u32 pi = threadIdx.x / lanes;
-    for (u32 u = threadIdx.x % lanes; u < units; u += lanes) {
-        const u32 c = u / V4, d = u % V4;
-        float M = -INFINITY, sum = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        const u32 s1 = min((pi + 1) * run, sq.ns);
-        for (u32 s0 = pi * run; s0 < s1; s0 += 8) {
-            u32x2v_t ml[8];
-            u32x4v_t v[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const u32 s = min(s0 + j, sq.ns - 1);
-                ml[j] = __builtin_amdgcn_raw_buffer_load_b64(rm, (s * CK_COLS + c) * 8, 0, TL_SC1);
-                v[j] = __builtin_amdgcn_raw_buffer_load_b128(ra, ((s * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
-            }
-            float Mn = M;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const u32 mb = ml[j][0];
-                Mn = fmaxf(Mn, s0 + j < s1 ? __uint_as_float(mb) : -INFINITY);
-            }
-            const float M0 = Mn == -INFINITY ? 0.f : Mn;
-            const float f0 = __builtin_amdgcn_exp2f(M - M0);
-            sum *= f0;
-            a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (s0 + j >= s1) break;
-                const u32 mb = ml[j][0], lb = ml[j][1];
-                const u32 v0 = v[j][0], v1 = v[j][1], v2 = v[j][2], v3 = v[j][3];
-                const float f = __builtin_amdgcn_exp2f(__uint_as_float(mb) - M0);
-                sum = fmaf(f, __uint_as_float(lb), sum);
-                a.x = fmaf(f, __uint_as_float(v0), a.x);
-                a.y = fmaf(f, __uint_as_float(v1), a.y);
-                a.z = fmaf(f, __uint_as_float(v2), a.z);
-                a.w = fmaf(f, __uint_as_float(v3), a.w);
-            }
-            M = Mn;
+    /* The last split of the group to arrive joins them all.  One workgroup reads
+     * some 0.1 MB in the time of a wait for memory: of many splits' rows, eight
+     * splits at a time are joined first, by the last of the eight to arrive, and
+     * the last of the last ones joins those.  The order of the sums is the splits',
+     * whoever comes last. */
+    auto arrive = [&](u32 *cnt, u32 of) -> bool {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh.last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
+            if (sh.last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        if (parts == 1) {
-            write(c, d, a, sum, M);
-        } else {
-            *(float4 *)&s_o[(pi * CK_COLS + c) * ROWF + 4 * d] = a;
-            if (d == 0) {
-                s_m[pi][c] = M;
-                s_l[pi][c] = sum;
+        __syncthreads();
+        return sh.last;
+    };
+    /* splits first, first + step, ... joined: `parts` threads to a float4 of the
+     * output, each with a run of the splits, eight of them requested at a time; then
+     * the parts through LDS, in order */
+    auto join = [&](u32 first, u32 step, u32 count, auto to) {
+        u32 parts = 1;
+        while (parts < NW && parts * 2 * units <= NT && parts * 8 < count) parts *= 2;
+        const u32 run = (count + parts - 1) / parts;
+        const u32 lanes = parts == 1 ? NT : NT / parts;
+        const u32 pi = threadIdx.x / lanes;
+        for (u32 u = threadIdx.x % lanes; u < units; u += lanes) {
+            const u32 c = u / V4, d = u % V4;
+            float M = -INFINITY, sum = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            const u32 s1 = min((pi + 1) * run, count);
+            for (u32 s0 = pi * run; s0 < s1; s0 += 8) {
+                u32x2v_t ml[8];
+                u32x4v_t v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const u32 s = first + step * min(s0 + j, count - 1);
+                    ml[j] = __builtin_amdgcn_raw_buffer_load_b64(rm, (s * CK_COLS + c) * 8, 0, TL_SC1);
+                    v[j] = __builtin_amdgcn_raw_buffer_load_b128(ra, ((s * CK_COLS + c) * D + 4 * d) * 4, 0, TL_SC1);
+                }
+                float Mn = M;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const u32 mb = ml[j][0];
+                    Mn = fmaxf(Mn, s0 + j < s1 ? __uint_as_float(mb) : -INFINITY);
+                }
+                const float M0 = Mn == -INFINITY ? 0.f : Mn;
+                const float f0 = __builtin_amdgcn_exp2f(M - M0);
+                sum *= f0;
+                a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (s0 + j >= s1) break;
+                    const u32 mb = ml[j][0], lb = ml[j][1];
+                    const u32 v0 = v[j][0], v1 = v[j][1], v2 = v[j][2], v3 = v[j][3];
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(mb) - M0);
+                    sum = fmaf(f, __uint_as_float(lb), sum);
+                    a.x = fmaf(f, __uint_as_float(v0), a.x);
+                    a.y = fmaf(f, __uint_as_float(v1), a.y);
+                    a.z = fmaf(f, __uint_as_float(v2), a.z);
+                    a.w = fmaf(f, __uint_as_float(v3), a.w);
+                }
+                M = Mn;
+            }
+            if (parts == 1) {
+                to(c, d, a, sum, M);
+            } else {
+                *(float4 *)&s_o[(pi * CK_COLS + c) * ROWF + 4 * d] = a;
+                if (d == 0) {
+                    s_m[pi][c] = M;
+                    s_l[pi][c] = sum;
+                }
             }
         }
-    }
-    if (parts > 1) {
+        if (parts == 1) return;
         __syncthreads();
         for (u32 u = threadIdx.x; u < units; u += NT) {
             const u32 c = u / V4, d = u % V4;
@@ -331,11 +337,22 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
                 a.z = fmaf(f, v.z, a.z);
                 a.w = fmaf(f, v.w, a.w);
             }
-            write(c, d, a, sum, M);
+            to(c, d, a, sum, M);
         }
+    };
+    const u32 n_cnt = sq.counters;
+    u32 *cnt = p.cnt + ((u64)sq.grp0 + (u64)group * n_cnt) * CK_CNT_PAD;
+    if (n_cnt > 1) {
+        const u32 s0 = split / CK_JOIN * CK_JOIN, of = min((u32)CK_JOIN, sq.ns - s0);
+        if (!arrive(cnt + (1 + split / CK_JOIN) * CK_CNT_PAD, of)) return;
+        /* a column's threads are of one wave, which has read its row before it writes it */
+        join(s0, 1, of, [&](u32 c, u32 d, float4 a, float sum, float M) { keep(s0, c, d, a, sum, M); });
+        if (!arrive(cnt, n_cnt - 1)) return;
+        join(0, CK_JOIN, n_cnt - 1, write);
+    } else {
+        if (!arrive(cnt, sq.ns)) return;
+        join(0, 1, sq.ns, write);
     }
-    if (threadIdx.x == 0)
-        __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 /* ---- many columns: 128 to a workgroup, K and V tiles shared through LDS ------
