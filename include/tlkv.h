@@ -417,7 +417,7 @@ int tl_qk_norm_append_q8(const tl_kv_layer_q8 *L, const tl_qk_norm_args *a,
  * A row that sees nothing gives zeros, and a log sum of -infinity.  Keys that
  * a row does not see have no part in it, whatever their K and V hold; one that
  * sees an infinity or NaN may come out as NaN (a Q8_0 element counts as an
- * infinity past the range of f16).  dst shares no floats with q. */
+ * infinity past the range of f16).  q, dst and lse share no floats. */
 typedef struct tl_chunk_attn_args {
     const float    *q;        /* device [rows][q_stride], rotated */
     float          *dst;      /* device [rows][q_stride] */
@@ -451,7 +451,7 @@ int tl_attn_chunks_ws(uint32_t n_kv_head, uint32_t head_dim, const tl_chunk_attn
  * sessions: for each chunk and each position j < pos + n
  *     weight[j] += sum over its rows and all heads of exp(s - lse)
  * with the scores and masks of tl_attn_chunks, whose lse these are (dst is not
- * used).  The order of the sums is fixed: equal calls give equal bits. */
+ * used).  The chunks' weights share no floats with each other, q or lse.  The order of the sums is fixed: equal calls give equal bits. */
 int tl_attn_weight(const tl_kv_layer *L, const tl_chunk_attn_args *a, const tl_chunk *chunks,
                    uint32_t n_chunk, void *stream);
 int tl_attn_weight_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a,
@@ -465,7 +465,8 @@ int tl_attn_weight_q8(const tl_kv_layer_q8 *L, const tl_chunk_attn_args *a,
  * one of larger pages the source rows of a tl_kv_copy into new pages), the
  * rows of the evicted positions in the order of their positions, and the kept
  * weights.  The pool's rows themselves are not touched.  After it the session
- * has `keep` positions, and rope_skip grows by len - keep. */
+ * has `keep` positions, and rope_skip grows by len - keep.  At most 4096
+ * sessions. */
 typedef struct tl_evict_seq {
     const float    *weight;   /* device [len] */
     const uint32_t *pages;    /* device: the session's page table; NULL = identity */
@@ -479,7 +480,7 @@ typedef struct tl_evict_seq {
     uint32_t       *rows;     /* device [keep]; NULL: not wanted */
     uint32_t       *freed;    /* device [len - keep]; NULL: not wanted */
     float          *weight_out; /* device [keep]; NULL: not wanted.  No output may overlap an
-                                   input or another output */
+                                   input or another output of the call */
 } tl_evict_seq;
 int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *stream);
 

@@ -72,6 +72,37 @@ def test_attn_args_refused(bad):
     assert L.tl_attn_chunks_q8(layer_q8(), attn(**bad), ch, n, None) == -1
 
 
+def test_lse_and_weight_apart():
+    """Outputs that lie over another buffer of the call."""
+    L, (ch, n) = tlkv.lib(), chunks(ONE)
+    q, rows = 1 << 30, 64 * 4096 * 4
+    for lse in (q, q + rows - 4, q - 64 * 32 * 4 + 4, 1 << 31, (1 << 31) + rows - 4):
+        assert L.tl_attn_chunks(layer(), attn(lse=lse), ch, n, None) == -1
+        assert L.tl_attn_chunks_q8(layer_q8(), attn(lse=lse), ch, n, None) == -1
+    for w in (q, q + rows - 4, q - 44, P, P + 64 * 32 * 4 - 4):
+        ch, n = chunks(dict(), dict(weight=w))
+        assert L.tl_attn_weight(layer(), attn(), ch, n, None) == -1
+        assert L.tl_attn_weight_q8(layer_q8(), attn(), ch, n, None) == -1
+
+
+def test_many_heads_refused():
+    """More q heads to a kv head than 32 bits hold columns of."""
+    one = layer(n_kv_head=1, head_dim=64)
+    L, (ch, n) = tlkv.lib(), chunks(dict(n=1, row=0))
+    for name in ("tl_attn_chunks", "tl_attn_weight"):
+        for heads in (1 << 16, (1 << 26) - 1):
+            a = attn(rows=1, n_head=heads, q_stride=heads * 64, q=1 << 40, dst=1 << 45)
+            assert getattr(L, name)(one, a, ch, n, None) == -2
+
+
+def test_many_chunks_out_of_order():
+    L = tlkv.lib()
+    cs = [dict(row=3 * (i * 1237 % 4096), n=3, weight=P * (64 + i)) for i in range(4096)]
+    for at, bad in ((17, dict(row=cs[4000]["row"] + 2)), (4095, dict(row=cs[9]["row"], n=1))):
+        ch, n = chunks(*(cs[:at] + [dict(cs[at], **bad)] + cs[at + 1:]))
+        assert L.tl_attn_chunks(layer(), attn(rows=3 * 4096 + 8, dst=1 << 45), ch, n, None) == -1
+
+
 def test_attn_workspace_refused():
     L, (ch, n) = tlkv.lib(), chunks(dict(pos=5000, n=1))
     need = ctypes.c_uint64()
@@ -151,3 +182,17 @@ def test_evict_refused(bad):
                               tlkv.EvictSeq(**a))
     assert tlkv.lib().tl_kv_evict(two, 2, None) == -1
     assert tlkv.lib().tl_kv_evict(None, 1, None) == -1
+
+
+def test_evict_sessions_apart():
+    """An output of one session over an input or an output of another."""
+    L = tlkv.lib()
+    a = dict(weight=P, pages=2 * P, len=100, keep=50, sink=4, recent=10, page_size=16, kept=4 * P,
+             rows=5 * P, freed=6 * P, weight_out=7 * P)
+    b = {k: v + 16 * P if v >= P else v for k, v in a.items()}
+    for bad in (dict(kept=P), dict(rows=2 * P), dict(freed=4 * P), dict(weight_out=6 * P + 196),
+                dict(weight=5 * P), dict(pages=6 * P + 196)):
+        assert L.tl_kv_evict((tlkv.EvictSeq * 2)(tlkv.EvictSeq(**a), tlkv.EvictSeq(**dict(b, **bad))), 2, None) == -1
+        many = [dict(b, **{k: v + 16 * P * i for k, v in b.items() if v >= P}) for i in range(1, 40)]
+        assert L.tl_kv_evict((tlkv.EvictSeq * 41)(*[tlkv.EvictSeq(**x) for x in many + [a, dict(b, **bad)]]), 41, None) == -1
+    assert L.tl_kv_evict((tlkv.EvictSeq * 1)(tlkv.EvictSeq(**a)), 4097, None) == -1

@@ -81,6 +81,12 @@ int tl_check_layer(const tl_kv_layer *L);
 int tl_check_layer_q8(const tl_kv_layer_q8 *L);
 LayerView tl_view_q8(const tl_kv_layer_q8 *L);
 bool tl_ranges_overlap(const void *a, u64 a_bytes, const void *b, u64 b_bytes);
+/* Does one of the intervals that are written overlap another one?  Sorts them. */
+struct TlSpan {
+    u64 at, end;
+    bool write;
+};
+bool tl_spans_clash(TlSpan *a, u32 n);
 
 /* ---- device ---------------------------------------------------------------- */
 

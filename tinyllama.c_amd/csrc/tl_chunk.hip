@@ -8,6 +8,7 @@
 #include "tl_chunk_launch.h"
 
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
 /* ------------------------------------------------------------------------ */
@@ -19,22 +20,33 @@ bool tl_ranges_overlap(const void *a, u64 a_bytes, const void *b, u64 b_bytes) {
     return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
 }
 
-/* do the intervals [at(i), at(i) + len(i)) of items with len > 0 overlap?
- * Rising ones (the usual order) are seen in one pass. */
+static int by_start(const void *a, const void *b) {
+    const u64 x = ((const TlSpan *)a)->at, y = ((const TlSpan *)b)->at;
+    return x < y ? -1 : x > y;
+}
+
+bool tl_spans_clash(TlSpan *a, u32 n) {
+    bool rising = true;
+    for (u32 i = 1; i < n && rising; i++) rising = a[i - 1].at <= a[i].at;
+    if (!rising) qsort(a, n, sizeof(*a), by_start);
+    u64 end = 0, written = 0;      /* of the intervals so far */
+    for (u32 i = 0; i < n; i++) {
+        if (a[i].at == a[i].end) continue;
+        if (a[i].at < (a[i].write ? end : written)) return true;
+        if (a[i].end > end) end = a[i].end;
+        if (a[i].write && a[i].end > written) written = a[i].end;
+    }
+    return false;
+}
+
+/* do the intervals [at(i), at(i) + len(i)) of chunks with len > 0 overlap? */
 template <class At, class Len>
 static bool any_overlap(u32 n, At at, Len len) {
-    u64 end = 0;
-    bool rising = true;
-    for (u32 i = 0; i < n && rising; i++) {
-        if (!len(i)) continue;
-        rising = at(i) >= end;
-        end = at(i) + len(i);
-    }
-    if (rising) return false;
+    TlSpan a[CK_MAX_CHUNKS];
+    u32 m = 0;
     for (u32 i = 0; i < n; i++)
-        for (u32 j = 0; j < i; j++)
-            if (len(i) && len(j) && at(i) < at(j) + len(j) && at(j) < at(i) + len(i)) return true;
-    return false;
+        if (len(i)) a[m++] = {at(i), at(i) + len(i), true};
+    return tl_spans_clash(a, m);
 }
 
 int tl_chunk_check(const LayerView &L, const tl_chunk *ch, u32 n_chunk, u32 rows, u32 page_size,
@@ -489,7 +501,7 @@ static int check_attn(const LayerView &L, const tl_chunk_attn_args *a, const tl_
         return tl_fail(TL_EINVAL, "attn_chunks: scale %g softcap %g", (double)a->scale, (double)a->softcap);
     const u64 gqa = a->n_head / L.n_kv_head;
     for (u32 i = 0; i < n_chunk; i++)
-        if (ch[i].n * gqa > 0xffffffffull / gqa - CK_WCOLS)
+        if (ch[i].n * gqa + CK_WCOLS > 0xffffffffull / gqa)
             return tl_fail(TL_ERANGE, "attn_chunks: %u rows of gqa %llu in a chunk", ch[i].n, (unsigned long long)gqa);
     if ((uintptr_t)a->ws & 15) return tl_fail(TL_EINVAL, "attn_chunks: workspace not 16-byte aligned");
     return TL_OK;
@@ -682,6 +694,10 @@ static int attn_chunks(const LayerView &L, const tl_chunk_attn_args *a, const tl
     const u32 width = a->n_head * L.head_dim;
     if (rows_overlap(a->rows, a->q, a->q_stride, width, a->dst, a->q_stride, width))
         return tl_fail(TL_EINVAL, "attn_chunks: dst overlaps q");
+    const u64 lse = (u64)a->rows * a->n_head * sizeof(float);
+    if (tl_ranges_overlap(a->lse, lse, a->q, span(a->rows, a->q_stride, width)) ||
+        tl_ranges_overlap(a->lse, lse, a->dst, span(a->rows, a->q_stride, width)))
+        return tl_fail(TL_EINVAL, "attn_chunks: lse overlaps q or dst");
     CkAttnParams p;
     fill_attn(p, L, a, shift);
     u64 parts;
@@ -785,6 +801,12 @@ static int attn_weight(const LayerView &L, const tl_chunk_attn_args *a, const tl
     if (any_overlap(n_chunk, [&](u32 i) { return (u64)(uintptr_t)ch[i].weight; },
                     [&](u32 i) { return ch[i].n ? ((u64)ch[i].pos + ch[i].n) * 4 : 0; }))
         return tl_fail(TL_EINVAL, "attn_weight: two chunks share weights");
+    for (u32 i = 0; i < n_chunk; i++) {
+        const u64 bytes = ch[i].n ? ((u64)ch[i].pos + ch[i].n) * sizeof(float) : 0;
+        if (tl_ranges_overlap(ch[i].weight, bytes, a->lse, (u64)a->rows * a->n_head * sizeof(float)) ||
+            tl_ranges_overlap(ch[i].weight, bytes, a->q, span(a->rows, a->q_stride, a->n_head * L.head_dim)))
+            return tl_fail(TL_EINVAL, "attn_weight: weight of chunk %u overlaps q or lse", i);
+    }
     CkAttnParams p;
     fill_attn(p, L, a, shift);
     u64 floats;

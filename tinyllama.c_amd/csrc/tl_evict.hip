@@ -4,6 +4,7 @@
  */
 #include "tl_chunk.h"
 
+#include <stdlib.h>
 #include <string.h>
 
 #define EV_MAX_SEQ 16
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(EV_THREADS) void evict_kernel(const EvParams p) {
 
 extern "C" int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *stream) {
     if (!n_seq) return TL_OK;
-    if (!seqs) return tl_fail(TL_EINVAL, "evict: null sessions");
+    if (!seqs || n_seq > CK_MAX_CHUNKS) return tl_fail(TL_EINVAL, "evict: 1..%d sessions", CK_MAX_CHUNKS);
     for (u32 i = 0; i < n_seq; i++) {
         const tl_evict_seq &q = seqs[i];
         if (!q.weight || !q.len || !q.keep || q.keep > q.len || (u64)q.sink + q.recent > q.keep ||
@@ -383,20 +384,29 @@ extern "C" int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *strea
                            q.keep, q.sink, q.recent);
         if (!q.page_size || (q.page_size & (q.page_size - 1)) || q.page_size > TL_MAX_PAGE)
             return tl_fail(TL_EINVAL, "evict: page size %u is no power of two up to %d", q.page_size, TL_MAX_PAGE);
-        const void *in[2] = {q.weight, q.pages};
-        const u64 in_n[2] = {q.len, ((u64)q.len + q.page_size - 1) / q.page_size};
-        const void *out[4] = {q.kept, q.rows, q.freed, q.weight_out};
-        const u64 out_n[4] = {q.keep, q.keep, (u64)q.len - q.keep, q.keep};
-        for (int a = 0; a < 4; a++) {
-            if (((uintptr_t)out[a] | (uintptr_t)in[a & 1]) & 3) return tl_fail(TL_EINVAL, "evict: session %u: alignment", i);
-            for (int b = 0; b < 2; b++)
-                if (tl_ranges_overlap(out[a], out_n[a] * 4, in[b], in_n[b] * 4))
-                    return tl_fail(TL_EINVAL, "evict: session %u: an output overlaps an input", i);
-            for (int b = 0; b < a; b++)
-                if (tl_ranges_overlap(out[a], out_n[a] * 4, out[b], out_n[b] * 4))
-                    return tl_fail(TL_EINVAL, "evict: session %u: outputs overlap", i);
-        }
+        if (((uintptr_t)q.weight | (uintptr_t)q.pages | (uintptr_t)q.kept | (uintptr_t)q.rows |
+             (uintptr_t)q.freed | (uintptr_t)q.weight_out) & 3)
+            return tl_fail(TL_EINVAL, "evict: session %u: alignment", i);
     }
+    /* no output over an input or another output, of any session */
+    TlSpan few[6 * EV_MAX_SEQ], *spans = n_seq > EV_MAX_SEQ ? (TlSpan *)malloc(6 * sizeof(TlSpan) * (size_t)n_seq) : few;
+    if (!spans) return tl_fail(TL_ENOMEM, "evict: %u sessions", n_seq);
+    u32 n = 0;
+    for (u32 i = 0; i < n_seq; i++) {
+        const tl_evict_seq &q = seqs[i];
+        auto add = [&](const void *at, u64 words, bool write) {
+            if (at && words) spans[n++] = {(u64)(uintptr_t)at, (u64)(uintptr_t)at + 4 * words, write};
+        };
+        add(q.weight, q.len, false);
+        add(q.pages, ((u64)q.len + q.page_size - 1) / q.page_size, false);
+        add(q.kept, q.keep, true);
+        add(q.rows, q.keep, true);
+        add(q.freed, (u64)q.len - q.keep, true);
+        add(q.weight_out, q.keep, true);
+    }
+    const bool clash = tl_spans_clash(spans, n);
+    if (spans != few) free(spans);
+    if (clash) return tl_fail(TL_EINVAL, "evict: an output overlaps an input or another output");
     const hipStream_t st = (hipStream_t)stream;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     bool asked = false;
