@@ -153,7 +153,11 @@ struct CkAppendParams {
  * rotation table goes to LDS once, then every group of D / 8 lanes takes head
  * rows of q, k and v in turn, eight elements to a lane: sum of squares over
  * the group by DPP, norm, rotation with the partner's elements (in the lane
- * for adjacent pairs, from lane +- rdim / 16 for half pairs), store. */
+ * for adjacent pairs, from memory again for half pairs), store.  Bound by the
+ * traffic, f32 in and f32 q, f16 K and V out: 2100 rows at 32/8/128 23.9 us, 4.1
+ * TB/s of 5.1 that a copy reaches; 16 rows at 8/4/256 5.2 us (a launch and one
+ * round trip).  One row to a workgroup keeps the rotation table to one row and a
+ * row's requests together; few rows share their heads out, up to 1024 workgroups. */
 template <int D, bool Q8>
 __global__ __launch_bounds__(256) void chunk_append_kernel(const CkAppendParams p) {
     constexpr u32 LPR = D / 8, GRP = 256 / LPR;

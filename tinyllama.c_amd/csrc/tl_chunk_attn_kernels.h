@@ -1,8 +1,18 @@
 /* tl_chunk_attn_kernels.h — attention of a batch of chunks over a paged cache.
  *
  * Columns: a chunk's rows x the q heads of one kv head (column = row * gqa +
- * head), 16 to a workgroup; a column's softmax runs in one pass over the keys
- * with a running maximum and sum. */
+ * head); a column's softmax runs in one pass over the keys with a running
+ * maximum and sum.  f32 accuracy on f16 matrix instructions: q, scaled by a power
+ * of two of its row, and the probabilities are pairs hi + lo of f16 (22 bits), K
+ * and V exact; a Q8_0 element, int8 x f16 scale, is a pair too (K = kh + kl; the
+ * product of the two low halves is below 2^-22 and left out).
+ *
+ * Few columns (narrow): 16 to a workgroup, whose waves take the tiles of 32 keys
+ * in turn, K and V straight from memory into the matrix operands' layout.  Bound
+ * by the read of K and V at long contexts (one session of 32782 keys at 32/8/128
+ * 30.6 us, 4.4 TB/s, with capped scores; 16 sessions of 512 to 8192 keys at 28/4/128
+ * 21.6 us), below some 5 us of work by the chain of look-up, tile, join: 4 sessions
+ * of 5 rows, 32/8/64, 10.8 us. */
 #pragma once
 #include "tl_chunk.h"
 
@@ -373,7 +383,15 @@ TL_DEV void ck_narrow(const CkAttnParams &p, const CkSeq &sq, CkNarrowShared<D, 
  * pairs), so that both operands are 16-byte reads, four requested ahead of the
  * matrix instructions.  16-byte units are permuted within a row so that 16
  * lanes' reads cover all banks.  A Q8_0 tile is kept as two planes, hi and lo,
- * both through registers (waves 0 and 1 K, waves 2 and 3 V). */
+ * both through registers (waves 0 and 1 K, waves 2 and 3 V).
+ *
+ * Bound by the matrix instructions (four products for two, because of the pairs)
+ * together with the seven vector ones that go with each of them: 512 rows of
+ * documents of up to 9000 tokens at 16384 keys, 32/8/128, 141-148 us with the join
+ * (8), 0.9 PFLOP/s of matrix work, matrix pipe busy half of the time.  A workgroup
+ * by itself needs 0.43 us of it per tile and takes 1.16 (head_dim 256: 0.85 and
+ * 1.62, its LDS reads as long as its matrix work), after some 8 us for the chain of
+ * arguments, look-ups, first tiles and the last stores. */
 typedef float f16_t __attribute__((ext_vector_type(16)));
 template <int MC>
 struct CkAcc {
@@ -839,7 +857,8 @@ __global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel
 
 /* A batch of both kinds, head_dim 64 and 128: prompts' chunks and single tokens
  * side by side in one launch, narrow workgroups of four waves.  (6 sessions of 1
- * to 200 rows over a Q8_0 cache at 32/8/128: 39.7 us one after the other.) */
+ * to 200 rows over a Q8_0 cache at 32/8/128: 29.1 us, of which the join 5; 39.7
+ * one after the other.) */
 template <int D, bool Q8, bool BIAS>
 __global__ __launch_bounds__(256, 2) void chunk_attn_both_kernel(const CkAttnParams p) {
     static_assert(CkWide<D, Q8>::NT == 256, "one workgroup size");
