@@ -612,6 +612,24 @@ def test_kv_evict(T, lens, keeps, holds, page):
         assert k[-1] == r[-1] == f[-1] == -7 and o[-1] == -7.0
 
 
+def test_kv_evict_between_split_attention(T):
+    """Long sessions, more than one launch takes, beside short ones, and attention with many splits
+    before and after on the same stream's workspace: each call gives what it gives alone."""
+    rng = np.random.default_rng(4)
+    lens = [8193 + 1111 * i if i % 5 else 100 + i for i in range(24)]
+    keeps = [n // 3 + 1 for n in lens]
+    w = [rng.standard_normal(n).astype(np.float32) for n in lens]
+    B = R.Batch(5, SHAPES["gemma"], [(5000, 8)], 16, False)
+    D = Dev(T, B)
+    base = D.attn(1 / 16)
+    for _ in range(2):
+        got = run_evict(T, w, [None] * 24, 1, lens, keeps, [(2, 50)] * 24)
+        for i, n in enumerate(lens):
+            kept, gone = R.evict(w[i], n, keeps[i], 2, 50)
+            assert np.array_equal(got[i][0][:-1], kept) and np.array_equal(got[i][2][:-1], gone)
+        assert all(np.array_equal(a, b) for a, b in zip(base, D.attn(1 / 16)))
+
+
 @pytest.mark.parametrize("value", [0.0, np.nan, np.inf, -np.inf])
 def test_kv_evict_all_alike(T, value):
     """Equal weights: the lower positions stay."""

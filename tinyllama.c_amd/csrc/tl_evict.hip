@@ -16,20 +16,22 @@
 #define EV_BINS 2048                        /* digits of 11, 11 and 10 bits */
 #define EV_LOW 1024
 #define EV_MAX_SEG EV_THREADS               /* segments of a session that several workgroups share */
-#define EV_CNT (2 * EV_BINS + EV_LOW)       /* their histograms, zero between calls */
 #define EV_SEGW (EV_LOW + 8)                /* scratch words of a segment: counts by the last digit */
-static_assert(EV_MAX_SEQ * EV_CNT <= TL_MERGE_MAX_GROUPS * TL_MERGE_PAD, "counters of a stream's workspace");
+#define EV_AUX (EV_BINS + EV_LOW + 8)       /* of a session: histograms of digits 1 and 2, (prefix, want) of 0 and 1 */
+static_assert(EV_MAX_SEQ * EV_BINS <= TL_MERGE_MAX_GROUPS * TL_MERGE_PAD, "counters of a stream's workspace");
 
 struct EvSeq {
     const float *w;
     const u32 *pages;
     u32 *kept, *rows, *freed;
     float *w_out;
-    u32 *cnt;                               /* EV_CNT words, zero between calls */
+    u32 *cnt;                               /* histogram of digit 0, zero between calls */
     u32 *seg;                               /* EV_SEGW words per segment */
+    u32 *aux;                               /* EV_AUX words */
     u32 len, keep, sink, recent, shift, wg0;
 };
 struct EvParams {
+    u32 wg0[CK_MAX_SEQ];                    /* seq[].wg0 side by side */
     EvSeq seq[EV_MAX_SEQ];
     u32 n_seq;
 };
@@ -198,42 +200,45 @@ __global__ __launch_bounds__(EV_THREADS) void evict_one_kernel(const EvParams p)
     ev_write(s, 0, k, pref, want, want == held, 0, 0, s_w, s_at);
 }
 
-TL_DEV const EvSeq &ev_mine(const EvParams &p) {
-    u32 i = 0;
-    while (i + 1 < p.n_seq && p.seq[i + 1].wg0 <= blockIdx.x) i++;
-    return p.seq[i];
-}
+/* histogram of digit d */
+TL_DEV u32 *ev_hist(const EvSeq &s, int d) { return d == 0 ? s.cnt : s.aux + (d == 1 ? 0 : EV_BINS); }
 
-/* the digits before DIGIT from the session's histograms, by every workgroup for itself */
+/* The digits before DIGIT: the last one from its histogram, by every workgroup
+ * for itself, those before it as the session's first workgroup left them in the
+ * launch before. */
 template <int DIGIT>
-TL_DEV u32 ev_prefix(const EvSeq &s, u32 &want, u32 &held, u32 *s_w, u32 *s_pick) {
-    uint2 h[3];
-    u32 pref = 0;
-    if constexpr (DIGIT > 0) h[0] = ev_bins<EV_BINS>(s.cnt);
-    if constexpr (DIGIT > 1) h[1] = ev_bins<EV_BINS>(s.cnt + EV_BINS);
-    if constexpr (DIGIT > 2) h[2] = ev_bins<EV_LOW>(s.cnt + 2 * EV_BINS);
+TL_DEV u32 ev_prefix(const EvSeq &s, u32 seg, u32 &want, u32 &held, u32 *s_w, u32 *s_pick) {
     want = s.keep;
-#pragma unroll
-    for (int d = 0; d < DIGIT; d++) {
-        u32 bin;
-        ev_pick(h[d].x, h[d].y, want, bin, held, s_w, s_pick);
-        pref = ev_join(pref, d, bin);
+    if constexpr (DIGIT == 0) return 0;
+    else {
+        u32 pref = 0, bin, *left = s.aux + EV_BINS + EV_LOW + 2 * (DIGIT - 1);
+        const uint2 h = ev_bins<(DIGIT == 3 ? EV_LOW : EV_BINS)>(ev_hist(s, DIGIT - 1));
+        if constexpr (DIGIT > 1) {
+            pref = left[-2];
+            want = left[-1];
+        }
+        ev_pick(h.x, h.y, want, bin, held, s_w, s_pick);
+        pref = ev_join(pref, DIGIT - 1, bin);
+        if (DIGIT < 3 && seg == 0 && threadIdx.x == 0) {
+            left[0] = pref;
+            left[1] = want;
+        }
+        return pref;
     }
-    return pref;
 }
 
 /* Longer sessions: a workgroup per EV_SEG positions, one launch per digit.  A
  * workgroup adds its LDS histogram to the session's (integer atomics); those of
  * the next launch find the digit from it, each for itself (one round trip with
  * their keys'; a last workgroup that did it for all cost three more: 43 us for
- * 131072 positions, so 20; five empty launches are 12).  The last digit's counts
+ * 131072 positions, so 17; four empty launches are 10).  The last digit's counts
  * are also kept by segment. */
 template <int DIGIT>
 __global__ __launch_bounds__(EV_THREADS) void evict_digit_kernel(const EvParams p) {
     constexpr u32 NB = DIGIT == 2 ? EV_LOW : EV_BINS;
     __shared__ __align__(8) u32 s_hist[EV_BINS];
     __shared__ u32 s_w[EV_WAVES], s_pick[3];
-    const EvSeq &s = ev_mine(p);
+    const EvSeq &s = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 seg = blockIdx.x - s.wg0, tid = threadIdx.x;
     float w[EV_PER];
     u32 k[EV_PER];
@@ -241,7 +246,11 @@ __global__ __launch_bounds__(EV_THREADS) void evict_digit_kernel(const EvParams 
     for (u32 e = 0; e < EV_PER; e++) w[e] = s.w[min(seg * EV_SEG + e * EV_THREADS + tid, s.len - 1)];
     *(uint2 *)&s_hist[2 * tid] = make_uint2(0, 0);
     u32 want, held;
-    const u32 pref = ev_prefix<DIGIT>(s, want, held, s_w, s_pick);
+    const u32 pref = ev_prefix<DIGIT>(s, seg, want, held, s_w, s_pick);
+    /* the next launches' histograms to zero, and the first one for the next call */
+    if (DIGIT == 0 && seg == 0)
+        for (u32 x = tid; x < EV_BINS + EV_LOW; x += EV_THREADS) s.aux[x] = 0;
+    if (DIGIT == 2 && seg == 0) *(uint2 *)&s.cnt[2 * tid] = make_uint2(0, 0);
     __syncthreads();
     u32 above = 0;
 #pragma unroll
@@ -253,7 +262,7 @@ __global__ __launch_bounds__(EV_THREADS) void evict_digit_kernel(const EvParams 
         above += DIGIT == 2 && k[e] >> 10 > pref;
     }
     __syncthreads();
-    u32 *hist = s.cnt + DIGIT * EV_BINS;
+    u32 *hist = ev_hist(s, DIGIT);
 #pragma unroll
     for (u32 e = 0; e < NB / EV_THREADS; e++) {
         const u32 n = s_hist[e * EV_THREADS + tid];
@@ -275,7 +284,7 @@ __global__ __launch_bounds__(EV_THREADS) void evict_digit_kernel(const EvParams 
 __global__ __launch_bounds__(EV_THREADS) void evict_write_kernel(const EvParams p) {
     __shared__ u32 s_w[EV_WAVES], s_pick[3], s_base[2];
     __shared__ u16 s_at[EV_SEG];
-    const EvSeq &s = ev_mine(p);
+    const EvSeq &s = p.seq[ck_find(p.wg0, p.n_seq, blockIdx.x)];
     const u32 tid = threadIdx.x, seg = blockIdx.x - s.wg0, j0 = seg * EV_SEG, p0 = j0 + tid * EV_PER;
     u32 k[EV_PER];
     float w[EV_PER];
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(EV_THREADS) void evict_write_kernel(const EvParams 
 #pragma unroll
     for (u32 e = 0; e < EV_PER; e++) k[e] = ev_order(s, p0 + e, w[e]);
     u32 want, held, total;
-    const u32 top = ev_prefix<3>(s, want, held, s_w, s_pick);
+    const u32 top = ev_prefix<3>(s, seg, want, held, s_w, s_pick);
     /* what the segments before this one hold: a thread each (at most EV_MAX_SEG) */
     const u32 bin = top & (EV_LOW - 1);
     const u32 *sw = s.seg + (u64)tid * EV_SEGW + bin;
@@ -298,11 +307,6 @@ __global__ __launch_bounds__(EV_THREADS) void evict_write_kernel(const EvParams 
     if (tid == 0) s_base[1] = total;
     __syncthreads();
     ev_write(s, j0, k, top, want, want == held, s_base[1], s_base[0], s_w, s_at);
-}
-
-/* the histograms back to zero, once the last launch that reads them is through */
-__global__ __launch_bounds__(EV_THREADS) void evict_clear_kernel(const EvParams p) {
-    for (u32 x = threadIdx.x; x < EV_CNT; x += EV_THREADS) p.seq[blockIdx.x].cnt[x] = 0;
 }
 
 /* Any length without a workspace (captured calls, sessions past EV_MAX_SEG
@@ -442,23 +446,24 @@ extern "C" int tl_kv_evict(const tl_evict_seq *seqs, uint32_t n_seq, void *strea
                 wgs += kind == 1 ? (q.len + EV_SEG - 1) / EV_SEG : 1;
             }
             if (!p.n_seq) break;
+            for (u32 j = 0; j < CK_MAX_SEQ; j++) p.wg0[j] = j < p.n_seq ? p.seq[j].wg0 : ~0u;
             if (kind == 0) {
                 hipLaunchKernelGGL(evict_one_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
             } else if (kind == 2) {
                 hipLaunchKernelGGL(evict_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
             } else {
                 TlWorkspace *w;
-                const int rc = tl_workspace_get(st, (size_t)wgs * EV_SEGW, 0, TL_MERGE_CNT_WORDS, &w);
+                const int rc = tl_workspace_get(st, (size_t)wgs * EV_SEGW + p.n_seq * EV_AUX, 0, TL_MERGE_CNT_WORDS, &w);
                 if (rc) return rc;
                 for (u32 j = 0; j < p.n_seq; j++) {
-                    p.seq[j].cnt = w->cnt + (size_t)j * EV_CNT;
+                    p.seq[j].cnt = w->cnt + (size_t)j * EV_BINS;
+                    p.seq[j].aux = (u32 *)w->acc + (size_t)wgs * EV_SEGW + j * EV_AUX;
                     p.seq[j].seg = (u32 *)w->acc + (size_t)p.seq[j].wg0 * EV_SEGW;
                 }
                 hipLaunchKernelGGL(evict_digit_kernel<0>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
                 hipLaunchKernelGGL(evict_digit_kernel<1>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
                 hipLaunchKernelGGL(evict_digit_kernel<2>, dim3(wgs), dim3(EV_THREADS), 0, st, p);
                 hipLaunchKernelGGL(evict_write_kernel, dim3(wgs), dim3(EV_THREADS), 0, st, p);
-                hipLaunchKernelGGL(evict_clear_kernel, dim3(p.n_seq), dim3(EV_THREADS), 0, st, p);
             }
             HIP_TRY(hipGetLastError());
         }

@@ -87,6 +87,8 @@ static int ws_grow(TlWorkspace *w, size_t acc_floats, size_t ml_pairs, size_t co
         if (hipMalloc((void **)&w->acc, cap * sizeof(float)) != hipSuccess)
             return tl_fail(TL_ENOMEM, "workspace: %zu floats", cap);
         HIP_TRY(hipMemset(w->acc, 0, cap * sizeof(float)));
+        /* not ordered before work on non-blocking streams by itself */
+        HIP_TRY(hipDeviceSynchronize());
         w->acc_cap = cap;
     }
     if (ml_pairs > w->ml_cap) {
