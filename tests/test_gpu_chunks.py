@@ -616,7 +616,7 @@ def test_kv_evict_between_split_attention(T):
     """Long sessions, more than one launch takes, beside short ones, and attention with many splits
     before and after on the same stream's workspace: each call gives what it gives alone."""
     rng = np.random.default_rng(4)
-    lens = [8193 + 1111 * i if i % 5 else 100 + i for i in range(24)]
+    lens = [8193 + 1111 * i if i % 5 else 200 + i for i in range(24)]
     keeps = [n // 3 + 1 for n in lens]
     w = [rng.standard_normal(n).astype(np.float32) for n in lens]
     B = R.Batch(5, SHAPES["gemma"], [(5000, 8)], 16, False)
