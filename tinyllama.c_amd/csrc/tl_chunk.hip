@@ -154,7 +154,7 @@ struct CkAppendParams {
  * rows of q, k and v in turn, eight elements to a lane: sum of squares over
  * the group by DPP, norm, rotation with the partner's elements (in the lane
  * for adjacent pairs, from memory again for half pairs), store.  Bound by the
- * traffic, f32 in and f32 q, f16 K and V out: 2100 rows at 32/8/128 23.9 us, 4.1
+ * traffic, f32 in and f32 q, f16 K and V out: 2100 rows at 32/8/128 23.3 us, 4.2
  * TB/s of 5.1 that a copy reaches; 16 rows at 8/4/256 5.2 us (a launch and one
  * round trip).  One row to a workgroup keeps the rotation table to one row and a
  * row's requests together; few rows share their heads out, up to 1024 workgroups. */
@@ -166,6 +166,19 @@ __global__ __launch_bounds__(256) void chunk_append_kernel(const CkAppendParams 
     const u32 r = blockIdx.x - sq.wg0;
     const u32 key = sq.pos + r;
     const u64 brow = (u64)sq.row + r;
+    const u32 e0 = (threadIdx.x % LPR) * 8;
+    const u32 units = p.n_head + 2 * p.c.n_kv;
+    auto row_of = [&](u32 u) -> const float * {
+        const u32 kv = p.n_head + p.c.n_kv;
+        return u < p.n_head ? p.q + brow * p.q_stride + (u64)u * D
+             : u < kv ? p.k + brow * p.kv_stride + (u64)(u - p.n_head) * D
+                      : p.v + brow * p.kv_stride + (u64)(u - kv) * D;
+    };
+    const u32 u0 = blockIdx.y * GRP + threadIdx.x / LPR;
+    /* the first head row is on its way while the table is made */
+    const float *src = row_of(min(u0, units - 1));
+    float4 a = *(const float4 *)(src + e0), b = *(const float4 *)(src + e0 + 4);
+    const u32 prow = ck_row(p.c, sq.pages, key);
     if (threadIdx.x < p.rdim / 2) {
         /* turns in 64 bits: the fraction is good at any position */
         const double turns = (double)(key + sq.rope_skip) * (exp2(-p.step * (double)threadIdx.x) * 0.15915494309189535);
@@ -173,17 +186,16 @@ __global__ __launch_bounds__(256) void chunk_append_kernel(const CkAppendParams 
         sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
         s_cs[threadIdx.x] = make_float2(c, s);
     }
-    const u32 prow = ck_row(p.c, sq.pages, key);
     __syncthreads();
-    const u32 e0 = (threadIdx.x % LPR) * 8;
-    const u32 units = p.n_head + 2 * p.c.n_kv;
     const u32 half = p.rdim >> 1;
-    for (u32 u = blockIdx.y * GRP + threadIdx.x / LPR; u < units; u += gridDim.y * GRP) {
+    for (u32 u = u0; u < units; u += gridDim.y * GRP) {
         const bool is_q = u < p.n_head, is_v = u >= p.n_head + p.c.n_kv;
         const u32 h = is_q ? u : is_v ? u - p.n_head - p.c.n_kv : u - p.n_head;
-        const float *src = is_q ? p.q + brow * p.q_stride : is_v ? p.v + brow * p.kv_stride : p.k + brow * p.kv_stride;
-        src += (u64)h * D;
-        const float4 a = *(const float4 *)(src + e0), b = *(const float4 *)(src + e0 + 4);
+        if (u != u0) {
+            src = row_of(u);
+            a = *(const float4 *)(src + e0);
+            b = *(const float4 *)(src + e0 + 4);
+        }
         float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         float ss = 0.f;
 #pragma unroll
