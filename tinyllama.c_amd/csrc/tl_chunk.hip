@@ -597,19 +597,29 @@ static bool plan_weight(WeightPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_
         s.wg0 = (u32)wgs[0];
         wgs[0] += ((u64)s.pos + s.n - s.part0 + run * CK_KEYS - 1) / (run * CK_KEYS);
     }
-    /* shares of 128 columns at least, as many as run at once */
+    /* Shares of the columns, in units of 128: those for which rounds of
+     * workgroups x (the largest share + what a workgroup costs by itself) is least.
+     * 512 rows over 4608 keys, 32/8/128 Q8_0, us: one share (144 workgroups) 102,
+     * three (432, two rounds) 82; f16, three (216) 61, six (432, two rounds) 67. */
     const u32 fill = head_dim == 64 && !q8 ? 512 : 256;
-    u64 per = (shares * n_kv + fill - 1) / fill;
-    if (per < 1) per = 1;
-    for (; blocks * n_kv <= fill; per++) {
+    u64 per = 1;
+    double least = 0;
+    for (u64 x = 1 + shares * n_kv / (4 * fill); pl.n[1]; x += 1 + x / 32) {
         u64 at_once = 0;
+        double most = 0;
         bool one = true;
         for (u32 i = 0; i < pl.n[1]; i++) {
-            const u64 parts = ((u64)pl.seq[1][i].n * gqa + 127) / 128;
-            at_once += (u64)pl.seq[1][i].ncb * n_kv * ((parts + per - 1) / per);
-            one = one && parts <= per;
+            const u64 parts = ((u64)pl.seq[1][i].n * gqa + 127) / 128, k = (parts + x - 1) / x;
+            at_once += (u64)pl.seq[1][i].ncb * n_kv * k;
+            most = (double)parts / k > most ? (double)parts / k : most;
+            one = one && k == 1;
         }
-        if (at_once <= fill || one) break;
+        const double cost = (double)((at_once + fill - 1) / fill) * (most + 0.55);
+        if (!least || cost < least) {
+            least = cost;
+            per = x;
+        }
+        if (one) break;
     }
     for (u32 i = 0; i < pl.n[1]; i++) {
         CkSeq &s = pl.seq[1][i];
