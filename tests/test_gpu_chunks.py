@@ -380,6 +380,37 @@ def test_attn_weight(T, shape, sizes, page, q8, opt):
     assert all(T.equal(a, b) for a, b in zip(w, w2))
 
 
+def mixed_batch(seed):
+    """A batch of any shapes, lengths and masks together."""
+    r = np.random.default_rng(1000 + seed)
+    shape = list(SHAPES)[r.integers(len(SHAPES))]
+    top = int(r.choice([3, 40, 150]))
+    sizes = [(int(r.choice([0, r.integers(1, 70), r.integers(70, 900), r.integers(900, 2500)])),
+              int(r.choice([0, 1, 1, r.integers(1, 1 + top)]))) for _ in range(r.integers(1, 7))]
+    if not any(n for _, n in sizes):
+        sizes[0] = (sizes[0][0], 1)
+    opt = {}
+    if r.random() < 0.4:
+        opt["window"] = int(r.integers(1, 600))
+    if r.random() < 0.4:
+        opt["prefix"] = [int(r.integers(0, p + n + 40)) for p, n in sizes]
+    if r.random() < 0.3:
+        opt["softcap"] = float(r.uniform(2, 40))
+    if r.random() < 0.3:
+        opt["slopes"] = True
+    if r.random() < 0.4:
+        opt["first"] = True
+    return shape, sizes, int(r.choice([1, 2, 16, 64])), bool(r.random() < 0.4), opt
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_mixed_batches(T, seed):
+    """Attention and weight of batches whose shapes, lengths and masks come together by chance."""
+    shape, sizes, page, q8, opt = mixed_batch(seed)
+    test_attn_chunks(T, shape, sizes, page, q8, opt)
+    test_attn_weight(T, shape, sizes, page, q8, opt)
+
+
 def test_attn_weight_unseen_rows_hold_anything(T):
     B = R.Batch(23, SHAPES["8b"], [(40, 3)], 16)
     last = B.phys(0, 42)
