@@ -473,6 +473,9 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
         for (u32 i = 0; i < pl.n[w]; i++) {
             CkSeq &s = pl.seq[w][i];
             u64 ns = (tiles[w][i] + per - 1) / per;
+            /* two tiles to a wave cost less than a join at head_dim 64: 4 sessions of 5 rows at
+             * 300 keys 7.8 us / 9.4; at 128 one of 500 keys 11.1 / 10.1 */
+            if (!w && !both && head_dim == 64 && tiles[w][i] <= 2 * CK_WAVES(64)) ns = 1;
             const u64 groups = (u64)s.ncb * n_kv;
             const u64 cols = (u64)s.n * gqa;
             const u32 counters = ck_join_counters((u32)ns, cols < CK_COLS ? (u32)cols : CK_COLS, head_dim,
