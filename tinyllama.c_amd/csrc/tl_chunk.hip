@@ -420,9 +420,13 @@ static bool all_narrow(const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 
 }
 
 /* As many splits as fill the chip (narrow: one workgroup to a CU, wide: two, at
- * head_dim 256 one; in one launch of both, up to head_dim 128, the narrow ones
- * are of half the size and take what the wide ones leave), none of fewer tiles
- * than a narrow workgroup has waves, or of fewer keys than 128 (wide). */
+ * head_dim 256 one), none of fewer tiles than a narrow workgroup has waves, or of
+ * fewer keys than 128 (wide).  In one launch of both, up to head_dim 128, the
+ * narrow ones are of half the size; a wide tile takes three times as long as one of
+ * theirs, so the 512 places are shared out by that, and the wide ones have 192 keys
+ * at least.  us, all places for the wide ones / shared: 24 sessions of 1 to 150
+ * rows at up to 6000 keys, 32/8/128, 70.9 / 44.4; 12 of up to 30 at 8000 49.9 / 40.7;
+ * 6 of up to 200 26.4 / 25.4; the worst of 30, 20 of up to 400 rows, 48.7 / 52.3. */
 static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, u32 gqa, u32 head_dim, bool q8,
                       u32 window) {
     pl.n[0] = pl.n[1] = pl.wgs[0] = pl.wgs[1] = pl.groups = 0;
@@ -454,9 +458,13 @@ static bool plan_attn(AttnPlan &pl, const tl_chunk *const *ch, u32 n, u32 n_kv, 
     const bool both = pl.n[0] && pl.n[1] && head_dim != 256;
     for (int w = 1; w >= 0; w--) {
         u32 fill = w && head_dim != 256 ? 512 : 256;
+        if (both && w) {
+            fill = (u32)(512.0 * 3 * total[1] / (3.0 * total[1] + total[0]));
+            if (fill < 64) fill = 64;
+        }
         if (both && !w) fill = pl.wgs[1] < 384 ? 512 - pl.wgs[1] : 128;
         u64 per = (total[w] + fill - 1) / fill, wgs = 0;
-        const u64 least = !w && head_dim != 256 && !both ? 8 : 4;
+        const u64 least = both ? (w ? 6 : 4) : !w && head_dim != 256 ? 8 : 4;
         if (per < least) per = least;
         /* the smallest share whose workgroups all run at once, if there is one */
         u64 all = 0, most = 0;

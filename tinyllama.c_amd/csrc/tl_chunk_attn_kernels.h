@@ -857,7 +857,7 @@ __global__ __launch_bounds__((CkWide<D, Q8>::NT), 2) void chunk_attn_wide_kernel
 
 /* A batch of both kinds, head_dim 64 and 128: prompts' chunks and single tokens
  * side by side in one launch, narrow workgroups of four waves.  (6 sessions of 1
- * to 200 rows over a Q8_0 cache at 32/8/128: 29.1 us, of which the join 5; 39.7
+ * to 200 rows over a Q8_0 cache at 32/8/128: 28.1 us, of which the join 5; 39.7
  * one after the other.) */
 template <int D, bool Q8, bool BIAS>
 __global__ __launch_bounds__(256, 2) void chunk_attn_both_kernel(const CkAttnParams p) {
