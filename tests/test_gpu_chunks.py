@@ -643,6 +643,13 @@ def test_kv_evict(T, lens, keeps, holds, page):
         assert k[-1] == r[-1] == f[-1] == -7 and o[-1] == -7.0
 
 
+@pytest.mark.parametrize("lens", [[9000, 100, 1, 8192, 2049], [1, 8193], [30, 40] * 7 + [20000, 8200],
+                                  [30, 40] * 8 + [20000], [5, 2048, 70000, 2047, 8191]])
+def test_kv_evict_short_beside_long(T, lens):
+    """Short sessions in the long ones' launches, where there is room, and beside them."""
+    test_kv_evict(T, lens, [n // 3 + 1 for n in lens], [(min(n // 9, 4), min(n // 9, 100)) for n in lens], 16)
+
+
 def test_kv_evict_between_split_attention(T):
     """Long sessions, more than one launch takes, beside short ones, and attention with many splits
     before and after on the same stream's workspace: each call gives what it gives alone."""
