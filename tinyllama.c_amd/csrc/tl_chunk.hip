@@ -383,7 +383,7 @@ struct AttnPlan {
  * columns.  Fitted to both sides of 120 shapes; us narrow / wide at 32/8/128: 9
  * rows at 6000 keys 17 / 34, 60 rows 36 / 38, 200 rows 117 / 62; 128 rows at 500
  * keys 13 / 24; a first prompt of 300 rows 24 / 22; 8 sessions of 100 rows at 1000
- * keys 103 / 54; 6 of 1 to 200 rows at 64 to 6000 keys 35 / 26. */
+ * keys 103 / 54; 6 of 1 to 200 rows at 64 to 6000 keys 35 / 25. */
 #define CK_WIDE_MIN 32
 struct AttnCost {
     float base, round, tile;     /* narrow */
